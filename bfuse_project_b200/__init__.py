@@ -19,7 +19,16 @@ MAX_ARGS, MAX_SHAPE = 6, 12
 # operator bodies
 OP_SOFTMAX_F32, OP_LAYERNORM_F32, OP_RMSNORM_BF16, OP_ROPE_BF16 = 0, 1, 2, 3
 OP_GEMM_F32_SIMT, OP_CONV2D_F32_SIMT, OP_GEMM_TF32, OP_GEMM_BF16, OP_CONV2D_TF32 = 4, 5, 6, 7, 8
-FLAG_CAUSAL = 1
+OP_GEMM_ACT_BF16, OP_RESIDUAL_NORM_BF16, OP_ATTENTION_BF16 = 9, 10, 11
+FLAG_CAUSAL, FLAG_MUL = 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
+NORM_AFTER, NORM_BEFORE = 1, 2
+STATUS_BAD_OFFSETS = -1
+
+
+def flag_act(act):
+    """Activation (ACT_*) in the epilogue of OP_GEMM_ACT_BF16."""
+    return int(act) << 4
 
 
 def flag_share(n):

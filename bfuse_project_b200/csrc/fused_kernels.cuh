@@ -18,6 +18,8 @@
 // that keeps the lighter operator's occupancy without starving the heavier body of registers.
 #pragma once
 
+#include <type_traits>
+
 #include "dispatch.h"
 #include "tile.h"
 
@@ -102,10 +104,15 @@ constexpr int cmin(int a, int b) { return a < b ? a : b; }
 // Minimum CTAs per SM the pair is compiled for.  Two memory-bound bodies: the larger of their two
 // wishes (occupancy is what hides HBM latency).  A memory-bound body next to a GEMM / conv body:
 // at most 4, so the heavier body is not squeezed below 64 registers per thread.
+// A memory-bound body may name the most it can be squeezed to (kMostBlocks).
+template <class Op, class = void>
+constexpr int kMostBlocksOf = 32;
+template <class Op>
+constexpr int kMostBlocksOf<Op, std::void_t<decltype(Op::kMostBlocks)>> = Op::kMostBlocks;
 template <class A, class B>
 constexpr int pair_min_blocks() {
-  return (A::kMemoryBound && B::kMemoryBound) ? cmax(A::kMinBlocks, B::kMinBlocks)
-                                              : cmin(4, cmax(A::kMinBlocks, B::kMinBlocks));
+  return cmin(cmin(kMostBlocksOf<A>, kMostBlocksOf<B>), (A::kMemoryBound && B::kMemoryBound) ? cmax(A::kMinBlocks, B::kMinBlocks)
+                                              : cmin(4, cmax(A::kMinBlocks, B::kMinBlocks)));
 }
 
 // Pairs of such bodies test the thread index before both bodies (see fused_block_kernel).

@@ -11,10 +11,11 @@
 #include "ops_simt.cuh"
 #include "ops_conv_umma.cuh"
 #include "ops_umma.cuh"
+#include "ops_attention.cuh"
 
 namespace bfuse {
 
-constexpr int kNumOps = 9;
+constexpr int kNumOps = 12;
 
 template <int I> struct OpAt;
 template <> struct OpAt<0> { using type = SoftmaxF32; };
@@ -26,8 +27,11 @@ template <> struct OpAt<5> { using type = ConvSimtF32; };
 template <> struct OpAt<6> { using type = GemmUmma<0>; };
 template <> struct OpAt<7> { using type = GemmUmma<1>; };
 template <> struct OpAt<8> { using type = ConvAnyTf32; };
+template <> struct OpAt<9> { using type = GemmUmma<1, true>; };
+template <> struct OpAt<10> { using type = ResidualNormBf16; };
+template <> struct OpAt<11> { using type = AttentionBf16; };
 
-template <int KIND> inline constexpr bool kGuardFirst<GemmUmma<KIND>> = true;
+template <int KIND, bool ACT> inline constexpr bool kGuardFirst<GemmUmma<KIND, ACT>> = true;
 
 struct PairEntry {
   PairLaunchFn block, thread, queue;

@@ -250,6 +250,114 @@ struct RmsNormBf16 {
   }
 };
 
+// ------------------------------------------------- norms after and before a block, gate, residual
+//   b' = N(b) * w_after (or b);   r = x + scale * gate * b';   y = N(r) * w_before
+// with N(v) = v / sqrt(mean(v^2) + eps): what lies between two blocks of a layer, in one pass over its rows.  x and b are
+// read once and stay in registers (in bf16, 8 values a register quad; r takes their place in fp32), r and y are written
+// once.  y is taken from r before its rounding to bf16.  Either norm, the gate and either output may be absent.
+// Any multiple of 8 columns: threads per row are a power of two and a thread's last vector may lie past the row.
+struct ResidualNormBf16 {
+  static constexpr int kRunRows = 1;
+  struct Params {
+    const uint16_t *x;      // [rows, cols] the residual stream
+    const uint16_t *b;      // [rows, cols] the block's output
+    const uint16_t *gate;   // [ceil(rows / gate_rows), cols], or nullptr
+    const uint16_t *w_after, *w_before;   // [cols], nullptr: that norm is absent
+    uint16_t *r, *y;        // either may be nullptr
+    int rows, cols;
+    int gate_rows;          // rows that share a row of the gate
+    float eps, scale;
+  };
+  static constexpr int kMaxThreads = 256;
+  static constexpr int kMinBlocks = 4;   // 64 registers: 32 of them a row's slice
+  static constexpr int kMostBlocks = 4;  // (pairs with lighter bodies keep them, see pair_min_blocks)
+  static constexpr bool kMemoryBound = true;
+  static constexpr bool kUsesTmem = false;
+  static constexpr int kMaxVec = 4;      // 8 bf16 per vector: rows of up to 8192
+
+  __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
+    const int tpr = c.bx, tsh = log2_of(tpr), lane = c.tid & (tpr - 1), row = c.vblock * c.by + (c.tid >> tsh);
+    const int nv = p.cols >> 3;   // vectors of a row
+    c.dependency_wait();
+    const bool live = row < p.rows;
+    const uint4 *br = reinterpret_cast<const uint4 *>(p.b + (size_t)row * p.cols), *xr = reinterpret_cast<const uint4 *>(p.x + (size_t)row * p.cols);
+    const uint4 *g4 = p.gate ? reinterpret_cast<const uint4 *>(p.gate + (size_t)(live ? row / p.gate_rows : 0) * p.cols) : nullptr;
+    const uint4 *wa4 = reinterpret_cast<const uint4 *>(p.w_after), *wb4 = reinterpret_cast<const uint4 *>(p.w_before);
+    // every load of the row is issued before the first use of any of them (see SoftmaxF32)
+    uint4 b[kMaxVec], x[kMaxVec];
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+      const int k = i * tpr + lane;
+      b[i] = make_uint4(0, 0, 0, 0), x[i] = make_uint4(0, 0, 0, 0);
+      if (k < nv && live) b[i] = ld_stream_u4(br + k);
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+      const int k = i * tpr + lane;
+      if (k < nv && live) x[i] = ld_stream_u4(xr + k);
+    }
+    for (int k = lane; k < nv && live; k += tpr) {
+      if (g4) prefetch_l1(g4 + k);
+      if (c.tid < tpr) {   // one row's worth of threads touches every line of the weight vectors
+        if (wa4) prefetch_l1(wa4 + k);
+        if (wb4) prefetch_l1(wb4 + k);
+      }
+    }
+    float rinv = p.scale;
+    if (wa4) {
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMaxVec; ++i) {
+        const uint32_t u[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = bf16x2_to_f2(u[j]);
+          q += f.x * f.x + f.y * f.y;
+        }
+      }
+      rinv = p.scale / sqrtf(row_reduce<OpSum>(q, c, tpr, 0) / (float)p.cols + p.eps);
+    }
+    float r[kMaxVec][8];
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+      const int k = i * tpr + lane;
+      const bool in = k < nv && live;
+      const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+      const uint4 wv = wa4 && in ? __ldg(wa4 + k) : one, gv = g4 && in ? __ldg(g4 + k) : one;
+      const uint32_t ub[4] = {b[i].x, b[i].y, b[i].z, b[i].w}, ux[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      const uint32_t uw[4] = {wv.x, wv.y, wv.z, wv.w}, ug[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 fb = bf16x2_to_f2(ub[j]), fx = bf16x2_to_f2(ux[j]), fw = bf16x2_to_f2(uw[j]), fg = bf16x2_to_f2(ug[j]);
+        r[i][2 * j] = fx.x + fb.x * rinv * fw.x * fg.x;
+        r[i][2 * j + 1] = fx.y + fb.y * rinv * fw.y * fg.y;
+        q += r[i][2 * j] * r[i][2 * j] + r[i][2 * j + 1] * r[i][2 * j + 1];
+      }
+      if (in && p.r)
+        st_stream_u4(reinterpret_cast<uint4 *>(p.r + (size_t)row * p.cols) + k,
+                     make_uint4(f2_to_bf16x2(r[i][0], r[i][1]), f2_to_bf16x2(r[i][2], r[i][3]), f2_to_bf16x2(r[i][4], r[i][5]), f2_to_bf16x2(r[i][6], r[i][7])));
+    }
+    if (!wb4) return;
+    const float yinv = 1.f / sqrtf(row_reduce<OpSum>(q, c, tpr, 1) / (float)p.cols + p.eps);
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+      const int k = i * tpr + lane;
+      if (k < nv && live) {
+        const uint4 wv = __ldg(wb4 + k);
+        const uint32_t uw[4] = {wv.x, wv.y, wv.z, wv.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 fw = bf16x2_to_f2(uw[j]);
+          o[j] = f2_to_bf16x2(r[i][2 * j] * yinv * fw.x, r[i][2 * j + 1] * yinv * fw.y);
+        }
+        st_stream_u4(reinterpret_cast<uint4 *>(p.y + (size_t)row * p.cols) + k, make_uint4(o[0], o[1], o[2], o[3]));
+      }
+    }
+  }
+};
+
 // ------------------------------------------------------------------------------------- RoPE
 // q[seq, heads, dim] bf16.  BlockDim = (chunks * head_groups, positions per CTA, 1) where a chunk
 // is 8 consecutive rotary pairs (dim / 16 chunks per head); a thread computes the 8 sin/cos of its

@@ -23,6 +23,8 @@
 #include <cuda.h>
 #include <float.h>
 
+#include <type_traits>
+
 #include "tile.h"
 
 namespace bfuse {
@@ -39,6 +41,7 @@ enum UmmaStatus : int {
   UMMA_WAIT_FULL_TIMEOUT = 0x102,
   UMMA_WAIT_ACC_TIMEOUT = 0x103,
   UMMA_WAIT_PEERS_TIMEOUT = 0x104,
+  UMMA_WAIT_OTHER_TIMEOUT = 0x105,
 };
 
 // bm: rows of A (and of the output tile) per CTA, 128 or 256
@@ -58,6 +61,9 @@ __device__ __forceinline__ void mbar_inval(uint32_t bar) {
 }
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
@@ -79,8 +85,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int *st
     if (ok) return true;
     if ((it & 1023u) == 1023u) {
       // once any wait of the launch has given up, the others follow at once: a failed launch then ends
-      // after about one second in all, not one second per CTA
-      if (status && *reinterpret_cast<volatile int *>(status) != 0) return false;
+      // after about one second in all, not one second per CTA (negative: refused data, and nothing to give up for)
+      if (status && *reinterpret_cast<volatile int *>(status) > 0) return false;
       const uint64_t now = global_ns();
       if (t0 == 0) t0 = now;
       if (now - t0 > 1000000000ull) {
@@ -220,6 +226,43 @@ struct GemmUmmaParams {
   int bm;            // output-tile height: 128, or 256 (two MMAs per k-step share the W tile; split == 1 only)
   long long *timeline;  // diagnostic: when non-null, CTA 0 records globaltimer marks here (see UmmaMark)
 };
+
+// The product with more in its epilogue: out = act(A W^T + bias) + other, or * other.  `other` has the output's shape, so
+// its tiles come and go in the same boxes.
+struct GemmActParams : GemmUmmaParams {
+  alignas(64) CUtensorMap map_other;   // as map_out, for loads
+  int has_other;                       // 0: no residual / gate
+  int mul;                             // 1: act(...) * other, 0: act(...) + other
+  int act;                             // BFUSE_ACT_*
+};
+
+enum GemmAct : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4 };
+
+// x / (1 + e^-z) in fp32; the quick quotient is good to 2 ulp (the output is rounded to bf16) and 0 where e^-z passes 2^126
+__device__ __forceinline__ float over_one_plus_exp(float x, float z) { return __fdividef(x, 1.f + exp2f(z * -1.4426950408889634f)); }
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+  if (ACT == ACT_RELU) return x > 0.f ? x : (x != x ? x : 0.f);
+  if (ACT == ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  if (ACT == ACT_GELU_TANH) return over_one_plus_exp(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));   // 1/2 (1 + tanh u) = 1 / (1 + e^-2u)
+  if (ACT == ACT_SILU) return over_one_plus_exp(x, x);
+  return x;
+}
+__device__ __forceinline__ void activate16(int act, float (&v)[16]) {
+  if (act == ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_RELU>(v[j]);
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_GELU>(v[j]);
+  } else if (act == ACT_GELU_TANH) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_GELU_TANH>(v[j]);
+  } else if (act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_SILU>(v[j]);
+  }
+}
 
 // marks of the diagnostic timeline (nanoseconds on the global timer), written by virtual block 0
 enum UmmaMark : int {
@@ -365,6 +408,92 @@ struct ChunkWriter {
   }
 };
 
+constexpr int kActBarOffset = 256;   // in the window's header: a barrier per epilogue warp and staging buffer
+constexpr int kActBars = 4;          // staging buffers of a warp at most (staging_plan: 64 bf16 columns a chunk, 256 a tile)
+
+// The writer of GemmUmma<KIND, true>: `other` is loaded into the very staging buffer that its chunk of the output leaves
+// from, so it costs no shared memory; the loads of all buffers are under way before the first chunk is worked on, and
+// the tile's lines were asked into L2 while the MMAs ran (o-projection of 512 tokens and other sizes: operators' table).
+struct ActWriter : ChunkWriter<1> {
+  const GemmActParams *pa;
+  uint32_t bar0;                  // this warp's barriers, one per staging buffer
+  int *status;
+  int col0, m0, per_half, total;  // first chunk's column and row; chunks of 128 rows; chunks in all
+  int next = 0, loaded = 0;       // chunks begun; chunks whose load has been issued
+
+  __device__ __forceinline__ void load(int q, int half_end) {   // lane 0: chunk q into its buffer, unless it is another half's
+    if (q >= total || q >= half_end) return;
+    const uint32_t s = (uint32_t)(q % nbuf), bar = bar0 + 8 * s;
+    mbar_expect_tx(bar, 4096u);
+    tma_load_3d(buf0 + s * 4096u, &pa->map_other, bar, col0 + (q % per_half) * nb_step, m0 + (q / per_half) * kUmmaBM, bz);
+  }
+  __device__ __forceinline__ void prefetch() const {   // one lane
+    if (!pa->has_other) return;
+    for (int q = 0; q < total; ++q)
+      asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(&pa->map_other),
+                   "r"(col0 + (q % per_half) * nb_step), "r"(m0 + (q / per_half) * kUmmaBM), "r"(bz)
+                   : "memory");
+  }
+  // the ring is idle: every buffer starts with its first chunk
+  __device__ __forceinline__ void start() {
+    if (!pa->has_other) return;
+    loaded = min(nbuf, min(per_half, total));
+    if (lane == 0)
+      for (int q = 0; q < loaded; ++q) load(q, per_half);
+    __syncwarp();
+  }
+  __device__ __forceinline__ uint32_t begin_chunk() {
+    const uint32_t buf = ChunkWriter<1>::begin_chunk();
+    if (pa->has_other) {
+      if (next >= loaded) {   // a buffer's later use: the whole group that is free now
+        const int half_end = (next / per_half + 1) * per_half, end = min(next + group, min(half_end, total));
+        if (lane == 0)
+          for (int q = next; q < end; ++q) load(q, half_end);
+        loaded = end;
+        __syncwarp();
+      }
+      mbar_wait(bar0 + 8 * (uint32_t)(next % nbuf), (next / nbuf) & 1, status, UMMA_WAIT_OTHER_TIMEOUT);
+      __syncwarp();
+    }
+    ++next;
+    return buf;
+  }
+  __device__ __forceinline__ void put16(uint32_t buf, int sub, int nb, float (&v)[16], const float *bias_tile) {
+    const float4 *b4 = reinterpret_cast<const float4 *>(bias_tile + (nb + sub * 16 - n_tile0));
+    const float4 ba = b4[0], bb = b4[1], bc = b4[2], bd = b4[3];
+    v[0] += ba.x, v[1] += ba.y, v[2] += ba.z, v[3] += ba.w;
+    v[4] += bb.x, v[5] += bb.y, v[6] += bb.z, v[7] += bb.w;
+    v[8] += bc.x, v[9] += bc.y, v[10] += bc.z, v[11] += bc.w;
+    v[12] += bd.x, v[13] += bd.y, v[14] += bd.z, v[15] += bd.w;
+    activate16(pa->act, v);
+    const uint32_t row = buf + (uint32_t)lane * 128u;
+    if (pa->has_other) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 o = ld_shared_f4(row + (uint32_t)(((sub * 2 + j) ^ (lane & 7)) * 16));
+        const float u[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = bf16x2_to_f2(__float_as_uint(u[i]));
+          float &a = v[8 * j + 2 * i], &b = v[8 * j + 2 * i + 1];
+          a = pa->mul ? a * f.x : a + f.x;
+          b = pa->mul ? b * f.y : b + f.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      st_shared_u4(row + (uint32_t)(((sub * 2 + j) ^ (lane & 7)) * 16), f2_to_bf16x2(v[8 * j], v[8 * j + 1]),
+                   f2_to_bf16x2(v[8 * j + 2], v[8 * j + 3]), f2_to_bf16x2(v[8 * j + 4], v[8 * j + 5]),
+                   f2_to_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+  }
+  // no load may be in flight when the window is handed on (a wait before the last chunk gave up)
+  __device__ __forceinline__ void drain() {
+    for (; next < loaded; ++next) mbar_wait(bar0 + 8 * (uint32_t)(next % nbuf), (next / nbuf) & 1, status, UMMA_WAIT_OTHER_TIMEOUT);
+    __syncwarp();
+  }
+};
+
 // staging buffers (per epilogue warp) and chunks per bulk group for `total` chunks when `free_bufs`
 // buffers fit: a buffer per chunk in groups of two (the stores of one pair run while the next pair
 // is staged, and nothing is reused), else two alternating half-groups of up to 4, else one buffer
@@ -383,9 +512,9 @@ __device__ __forceinline__ void staging_plan(int free_bufs, int total, int &nbuf
 // its MMAs, so every ring is free) each CTA pushes its partials straight from tensor memory into
 // the owners' shared memory; an owner waits on its mbarrier, which counts the delivered bytes,
 // sums the k-slices in order (deterministic) and stores the chunk through `w`.
-template <int KIND>
+template <int KIND, class Writer>
 __device__ __forceinline__ void umma_split_reduce(const TileCtx &c, int BN, int split, int kslice, uint32_t tiles, uint32_t recv_bar,
-                                                  uint32_t tmem_row, bool acc_ok, ChunkWriter<KIND> &w, int n0,
+                                                  uint32_t tmem_row, bool acc_ok, Writer &w, int n0,
                                                   const float *bias_tile, long long *tl) {
   constexpr int kElem = KIND == 0 ? 4 : 2, kOutCols = 128 / kElem, kSub = kOutCols / 16;
   constexpr uint32_t kChunkPartial = (uint32_t)kOutCols * kUmmaBM * 4;
@@ -452,9 +581,12 @@ __device__ __forceinline__ void umma_split_reduce(const TileCtx &c, int BN, int 
   mark(MARK_REDUCED, c.tid == 0);
 }
 
-template <int KIND>
+// ACT: with activation and a residual or gate in the epilogue (bf16)
+template <int KIND, bool ACT = false>
 struct GemmUmma {
-  using Params = GemmUmmaParams;
+  static_assert(!ACT || KIND == 1, "the activating epilogue is built for bf16");
+  using Params = typename std::conditional<ACT, GemmActParams, GemmUmmaParams>::type;
+  using Writer = typename std::conditional<ACT, ActWriter, ChunkWriter<KIND>>::type;
   static constexpr int kMaxThreads = kUmmaThreads;
   static constexpr int kMinBlocks = 1;
   static constexpr bool kMemoryBound = false;
@@ -514,7 +646,7 @@ struct GemmUmma {
     // Tensor memory first: the SM starts its next CTA of this kernel only when this one has given up
     // its permit to allocate, so every instruction before that delays a co-resident CTA.  A tile
     // entirely above the diagonal of a causal product needs no accumulator.
-    const bool masked_tile = p.causal && n0 > m0 + BM - 1;
+    const bool masked_tile = !ACT && p.causal && n0 > m0 + BM - 1;
     if (warp == 5) {
       if (!c.tmem_given) {   // (a persistent CTA of the work queue holds its columns already)
         if (!masked_tile) tmem_alloc(smem_u32(tmem_slot), BN * halves);
@@ -531,8 +663,17 @@ struct GemmUmma {
     const int free_bufs = (stages * kStageBytes - (int)(staging - tiles)) / kUmmaStagingBytes;
     int nbuf, group;
     staging_plan(free_bufs, max_owned, nbuf, group);
-    ChunkWriter<KIND> w{&p.map_out, p.M, p.N, p.causal, staging + (uint32_t)(quad * nbuf) * 4096u, nbuf, lane, 0, m0 + quad * 32, bz, n0,
-                        split * kOutCols, group};
+    Writer w = Writer{ChunkWriter<KIND>{&p.map_out, p.M, p.N, p.causal, staging + (uint32_t)(quad * nbuf) * 4096u, nbuf, lane, 0, m0 + quad * 32, bz, n0,
+                                        split * kOutCols, group}};
+    if constexpr (ACT) {
+      w.pa = &p;
+      w.bar0 = full0 + kActBarOffset + 8 * kActBars * quad;
+      w.status = c.status;
+      w.col0 = n0 + (split > 1 ? kslice * kOutCols : 0);
+      w.m0 = m0 + quad * 32;
+      w.per_half = split > 1 ? max(0, (chunks - kslice + split - 1) / split) : chunks;
+      w.total = w.per_half * halves;
+    }
     long long *const tl = (p.timeline && c.vblock == 0) ? p.timeline : nullptr;
     auto mark = [&](int what, bool who) {
       if (tl && who) tl[what] = (long long)global_ns();
@@ -580,6 +721,7 @@ struct GemmUmma {
         mbar_init(acc_bar, 1);
         mbar_init(recv_bar, 1);
       }
+      if (ACT && lane < 4 * kActBars) mbar_init(full0 + kActBarOffset + 8 * lane, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -655,10 +797,16 @@ struct GemmUmma {
       // the epilogue warps are idle during the main loop: they fetch the tile's bias slice meanwhile
       // (only they read it, after their own named-barrier-free hand-off below)
       for (int i = c.tid; i < BN; i += 128) bias_tile[i] = (p.bias && n0 + i < p.N) ? __ldg(p.bias + n0 + i) : 0.f;
+      if constexpr (ACT) {
+        if (lane == 0) w.prefetch();
+      }
       asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory");  // the four epilogue warps only (ids 9 / 10)
       acc_ok = mbar_wait(acc_bar, 0, c.status, UMMA_WAIT_ACC_TIMEOUT);
       tc_fence_after();
       mark(MARK_ACC_READY, c.tid == 0);
+      if constexpr (ACT) {
+        if (acc_ok) w.start();
+      }
       if (acc_ok && split == 1) {
 #pragma unroll 1
         for (int h = 0; h < halves; ++h) {  // accumulator h holds output rows [m0 + 128 h, +128)
@@ -690,6 +838,9 @@ struct GemmUmma {
       }
     }
     if (split > 1) umma_split_reduce<KIND>(c, BN, split, kslice, tiles, recv_bar, tmem_row, acc_ok, w, n0, bias_tile, tl);
+    if constexpr (ACT) {
+      if (warp < 4) w.drain();
+    }
     tc_fence_before();
     c.sync();
     if (warp == 5 && !c.tmem_given) tmem_dealloc(tmem_acc, BN * halves);
@@ -701,6 +852,7 @@ struct GemmUmma {
         mbar_inval(recv_bar);
       }
     }
+    if (ACT && c.persistent && c.tid < 4 * kActBars) mbar_inval(full0 + kActBarOffset + 8 * c.tid);
     mark(MARK_END, c.tid == 0);
   }
 };

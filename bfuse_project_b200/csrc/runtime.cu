@@ -209,6 +209,57 @@ bool planes_pay(const int *s, int ohw, int tiles, int split, int share, int sm) 
   return planes < gathered;
 }
 
+bool is_gemm_umma(int op) { return op == BFUSE_OP_GEMM_TF32 || op == BFUSE_OP_GEMM_BF16 || op == BFUSE_OP_GEMM_ACT_BF16; }
+
+// ---- residual norm: shape = rows, cols, norms (BFUSE_NORM_*), rows that share a row of the gate (0: all) ----
+
+const char *residual_norm_problem(const bfuse_kernel_desc &d) {
+  const int *s = d.shape;
+  if (s[0] <= 0 || s[1] <= 0) return "rows and cols must be positive";
+  if (s[1] % 8 || s[1] > 8 * ResidualNormBf16::kMaxVec * 256) return "cols must be a multiple of 8, at most 8192";
+  if (s[2] < 0 || s[2] > (BFUSE_NORM_AFTER | BFUSE_NORM_BEFORE)) return "shape[2] (norms) must be a sum of BFUSE_NORM_*";
+  if (s[3] < 0) return "shape[3] (rows that share a row of the gate) must not be negative";
+  return nullptr;
+}
+// Threads per row: the fewest, from 8, that leave a thread at most two vectors of 8 values, 256 at most.
+int residual_norm_threads(int cols) {
+  int tpr = 8;
+  while (tpr < 256 && cols > 16 * tpr) tpr *= 2;
+  return tpr;
+}
+
+// ---- attention: shape = seqs, total_q, total_kv, heads, kv heads, dim, q stride, kv stride, key slices ----
+
+const char *attention_problem(const bfuse_kernel_desc &d) {
+  const int *s = d.shape;
+  if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0) return "sequences and their tokens must be positive";
+  if (s[3] <= 0 || s[4] <= 0 || s[3] % s[4] || s[3] / s[4] > kAttnRows) return "query heads must be a multiple of the kv heads, at most 128 times them";
+  if (s[5] <= 0 || s[5] % 8 || s[5] > 128) return "dim must be a multiple of 8, at most 128";
+  if (s[6] < 0 || s[7] < 0 || s[6] % 8 || s[7] % 8) return "strides must be multiples of 8 elements";
+  if ((s[6] && s[6] < (long long)s[3] * s[5]) || (s[7] && s[7] < (long long)s[4] * s[5])) return "a stride is shorter than a token's heads";
+  if (s[8] != 0 && s[8] != 1 && s[8] != 2 && s[8] != 4 && s[8] != 8) return "shape[8] (key slices) must be 1, 2, 4 or 8";
+  if (!(d.fparam[0] > 0.f) || !(d.fparam[0] < 1e30f)) return "the scale must be positive and finite";
+  const int positions = kAttnRows / (s[3] / s[4]);
+  const long long tiles = ((long long)s[1] + (long long)s[0] * (positions - 1)) / positions;
+  if (tiles * s[4] * 8 > 0x7fffffffLL) return "more tiles than a grid holds";
+  return nullptr;
+}
+// tiles at most: sum of ceil(len / P) over the sequences
+long long attention_tiles(const int *s) {
+  const int positions = kAttnRows / (s[3] / s[4]);
+  return ((long long)s[1] + (long long)s[0] * (positions - 1)) / positions;
+}
+int attention_min_stages(int dim, int split) { return std::max(2, ceil_div(attn_join_bytes(dim, split), attn_tile_bytes(dim)) - 1); }
+// Slices of a tile's keys: while the tiles alone leave SMs idle and every slice keeps two blocks of the average sequence.
+// Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
+int attention_slices(const int *s, int share, int sm) {
+  if (s[8] > 0) return s[8];
+  const long long base = attention_tiles(s) * s[4] * share, blocks = ceil_div(s[2], s[0] * kAttnKeys);
+  for (int split = share == 1 ? 8 : 4; split > 1; split = share == 1 ? split / 2 : 1)
+    if (base * split <= 2 * sm && blocks >= 2 * split) return split;
+  return 1;
+}
+
 int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *err) {
   const int *s = d->shape;
   auto set = [&](int gx, int gy, int gz, int bx, int by, size_t smem, int nargs) {
@@ -235,6 +286,22 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       if (s[0] <= 0 || !tpr) { *err = "rmsnorm: cols must be a multiple of 8 * (power-of-two threads per row)"; return BFUSE_ERR_SHAPE; }
       const int rpc = std::max(1, 256 / tpr);
       set(ceil_div(s[0], rpc), 1, 1, tpr, rpc, 256, 3);
+      return BFUSE_OK;
+    }
+    case BFUSE_OP_RESIDUAL_NORM_BF16: {
+      if (const char *m = residual_norm_problem(*d)) { *err = std::string("residual norm: ") + m; return BFUSE_ERR_SHAPE; }
+      const int tpr = residual_norm_threads(s[1]), rpc = std::max(1, 256 / tpr);
+      set(ceil_div(s[0], rpc), 1, 1, tpr, rpc, 256, 6);
+      return BFUSE_OK;
+    }
+    case BFUSE_OP_ATTENTION_BF16: {
+      if (const char *m = attention_problem(*d)) { *err = std::string("attention: ") + m; return BFUSE_ERR_SHAPE; }
+      const long long tiles = attention_tiles(s);
+      const int split = attention_slices(s, share, sm);
+      d->shape[8] = split;
+      const int budget = (long long)share * tiles * s[4] * split <= sm ? 200 * 1024 : 110 * 1024;
+      const int stages = std::max(attention_min_stages(s[5], split), std::min(kAttnMaxStages, (budget - kUmmaHeaderBytes) / attn_tile_bytes(s[5]) - 1));
+      set(split * s[4], (int)tiles, 1, kAttnThreads, 1, attn_smem_bytes(s[5], stages), 6);
       return BFUSE_OK;
     }
     case BFUSE_OP_ROPE_BF16: {
@@ -344,7 +411,8 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       return BFUSE_OK;
     }
     case BFUSE_OP_GEMM_TF32:
-    case BFUSE_OP_GEMM_BF16: {
+    case BFUSE_OP_GEMM_BF16:
+    case BFUSE_OP_GEMM_ACT_BF16: {
       if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0 || s[3] <= 0) { *err = "gemm: batch, M, N, K must be positive"; return BFUSE_ERR_SHAPE; }
       const int eb = d->op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
       int bn = s[4], split = s[5], bm = s[6], q;
@@ -379,7 +447,7 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       const int budget = (bn == 256 || share * ctas <= sm) ? 200 * 1024 : 100 * 1024;
       int stages = std::min({q, kUmmaMaxStages, (budget - kUmmaHeaderBytes) / umma_stage_bytes(bn, bm)});
       stages = std::max({stages, 1, umma_min_stages(bn, split, eb, bm)});
-      set(split * ceil_div(s[1], bm), ceil_div(s[2], bn), s[0], kUmmaThreads, 1, umma_smem_bytes(bn, stages, bm), 4);
+      set(split * ceil_div(s[1], bm), ceil_div(s[2], bn), s[0], kUmmaThreads, 1, umma_smem_bytes(bn, stages, bm), d->op == BFUSE_OP_GEMM_ACT_BF16 ? 5 : 4);
       return BFUSE_OK;
     }
     default:
@@ -425,6 +493,32 @@ int describe_args(const bfuse_kernel_desc &d, ArgInfo *a, std::string *err) {
       a[3] = {n(e * s[0] * s[1] * s[2]), 1, 0};
       return 4;
     }
+    case BFUSE_OP_GEMM_ACT_BF16:
+      a[0] = {n(2LL * s[0] * s[1] * s[3]), 0, 0};
+      a[1] = {n(2LL * s[0] * s[2] * s[3]), 0, 0};
+      a[2] = {n(4LL * s[2]), 0, 1};
+      a[3] = {n(2LL * s[0] * s[1] * s[2]), 0, 1};
+      a[4] = {n(2LL * s[0] * s[1] * s[2]), 1, 0};
+      return 5;
+    case BFUSE_OP_RESIDUAL_NORM_BF16: {
+      const int norms = (s[2] & BFUSE_NORM_AFTER ? 1 : 0) + (s[2] & BFUSE_NORM_BEFORE ? 1 : 0);
+      a[0] = {n(2LL * s[0] * s[1]), 0, 0};
+      a[1] = {n(2LL * s[0] * s[1]), 0, 0};
+      a[2] = {n(2LL * s[1] * (s[3] > 0 ? ceil_div(s[0], s[3]) : 1)), 0, 1};
+      a[3] = {n(2LL * s[1] * norms), 0, norms == 0};
+      a[4] = {n(2LL * s[0] * s[1]), 1, (s[2] & BFUSE_NORM_BEFORE) != 0};
+      a[5] = {n(2LL * s[0] * s[1]), 1, !(s[2] & BFUSE_NORM_BEFORE)};
+      return 6;
+    }
+    case BFUSE_OP_ATTENTION_BF16: {
+      const long long qs = s[6] ? s[6] : (long long)s[3] * s[5], ks = s[7] ? s[7] : (long long)s[4] * s[5];
+      a[0] = {n(2LL * ((s[1] - 1) * qs + (long long)s[3] * s[5])), 0, 0};
+      a[1] = a[2] = {n(2LL * ((s[2] - 1) * ks + (long long)s[4] * s[5])), 0, 0};
+      a[3] = {n(4LL * (s[0] + 1)), 0, 0};
+      a[4] = {n(4LL * (s[0] + 1)), 0, 1};
+      a[5] = {n(2LL * s[1] * s[3] * s[5]), 1, 0};
+      return 6;
+    }
     case BFUSE_OP_CONV2D_F32_SIMT:
     case BFUSE_OP_CONV2D_TF32: {
       const int oh = conv_out(s[2], s[5], s[7], s[8]), ow = conv_out(s[3], s[6], s[7], s[8]);
@@ -453,6 +547,20 @@ int encode_map(bfuse_context *ctx, CUtensorMap *map, int dtype_bytes, const void
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ctx, BFUSE_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return BFUSE_OK;
+}
+
+// {dim (contiguous), heads, tokens} of one of attention's tensors with a box of 64 elements x heads x tokens, 128B swizzle
+int encode_heads(bfuse_context *ctx, CUtensorMap *map, const void *base, int dim, int heads, int tokens, long long token_stride, int box_heads,
+                 int box_tokens) {
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)dim * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ctx, BFUSE_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed (" + std::to_string((int)r) + ")");
   return BFUSE_OK;
 }
 
@@ -611,9 +719,55 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       std::memcpy(k.params, &p, sizeof(p));
       return BFUSE_OK;
     }
+    case BFUSE_OP_RESIDUAL_NORM_BF16: {
+      if (const char *m = residual_norm_problem(d)) return shape_err(m);
+      const int tpr = kd.bx, rpc = kd.by;
+      if (!is_pow2(tpr) || kd.bz != 1) return shape_err("BlockDim must be (power-of-two threads per row, rows per CTA, 1)");
+      if (s[1] > 8 * ResidualNormBf16::kMaxVec * tpr) return shape_err("cols do not fit the per-thread vector budget");
+      if (kd.gy != 1 || kd.gz != 1 || (long long)kd.gx * rpc < s[0]) return shape_err("GridDim.X * rows per CTA must cover the rows");
+      if (tpr > 32 && k.smem < 256) return shape_err("rows wider than a warp need 256 bytes of shared memory");
+      const bool after = s[2] & BFUSE_NORM_AFTER, before = s[2] & BFUSE_NORM_BEFORE;
+      if (!before && a[5]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": y is the output of the norm before the next block, which shape[2] leaves out");
+      if (!a[4] && !a[5]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": missing argument buffer");
+      const uint16_t *w = (const uint16_t *)a[3];
+      ResidualNormBf16::Params p{(const uint16_t *)a[0], (const uint16_t *)a[1], (const uint16_t *)a[2], after ? w : nullptr,
+                                 before ? w + (after ? s[1] : 0) : nullptr, (uint16_t *)a[4], (uint16_t *)a[5], s[0], s[1],
+                                 s[3] > 0 ? s[3] : s[0], d.fparam[0], d.fparam[1]};
+      std::memcpy(k.params, &p, sizeof(p));
+      return BFUSE_OK;
+    }
+    case BFUSE_OP_ATTENTION_BF16: {
+      if (const char *m = attention_problem(d)) return shape_err(m);
+      const int split = s[8] > 0 ? s[8] : 1, group = s[3] / s[4], positions = kAttnRows / group;
+      if (kd.bx != kAttnThreads || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1)");
+      if (kd.gx != split * s[4] || kd.gy != attention_tiles(s) || kd.gz != 1)
+        return shape_err("GridDim must be (key slices * kv heads, (total_q + seqs * (P - 1)) / P, 1) with P = 128 / (heads / kv heads) positions a tile");
+      if (k.smem < (size_t)attn_smem_bytes(s[5], attention_min_stages(s[5], split)))
+        return shape_err("shared memory below the queries and two blocks of keys or values (and, with key slices, what they exchange)");
+      k.cluster = split;
+      AttentionParams p;
+      std::memset(&p, 0, sizeof(p));
+      const long long qs = s[6] ? s[6] : (long long)s[3] * s[5], ks = s[7] ? s[7] : (long long)s[4] * s[5];
+      int rc = encode_heads(ctx, &p.map_q, a[0], s[5], s[3], s[1], qs, group, positions);
+      if (!rc) rc = encode_heads(ctx, &p.map_k, a[1], s[5], s[4], s[2], ks, 1, kAttnKeys);
+      if (!rc) rc = encode_heads(ctx, &p.map_v, a[2], s[5], s[4], s[2], ks, 1, kAttnKeys);
+      if (rc) return rc;
+      p.cu_q = (const int *)a[3], p.cu_kv = (const int *)(a[4] ? a[4] : a[3]);
+      p.out = (uint16_t *)a[5];
+      p.seqs = s[0], p.total_q = s[1], p.total_kv = s[2], p.heads = s[3], p.kv_heads = s[4], p.dim = s[5];
+      p.group = group, p.positions = positions;
+      p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL), p.split = split;
+      p.stages = std::min<int>(kAttnMaxStages, (int)((k.smem - kUmmaHeaderBytes) / attn_tile_bytes(s[5])) - 1);
+      p.scale_log2 = d.fparam[0] * 1.4426950408889634f;
+      static_assert(sizeof(p) <= kParamsBytes, "parameter block too small");
+      std::memcpy(k.params, &p, sizeof(p));
+      return BFUSE_OK;
+    }
     case BFUSE_OP_GEMM_TF32:
-    case BFUSE_OP_GEMM_BF16: {
+    case BFUSE_OP_GEMM_BF16:
+    case BFUSE_OP_GEMM_ACT_BF16: {
       const int eb = d.op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
+      const bool act = d.op == BFUSE_OP_GEMM_ACT_BF16;
       const int bn = s[4], split = s[5] > 0 ? s[5] : 1, bm = s[6] > 0 ? s[6] : kUmmaBM;
       if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0 || s[3] <= 0) return shape_err("batch, M, N, K must be positive");
       if (bn != 32 && bn != 64 && bn != 128 && bn != 256) return shape_err("shape[4] (BN) must be 32, 64, 128 or 256");
@@ -630,16 +784,27 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if (k.smem < (size_t)umma_smem_bytes(bn, umma_min_stages(bn, split, eb, bm), bm))
         return shape_err("shared memory below the store buffers (and, for a split GEMM, the receive area of the k-slices)");
       k.cluster = split;
-      GemmUmmaParams p;
+      if (act && (d.flags & BFUSE_FLAG_CAUSAL)) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": no causal mask in this epilogue");
+      if (act && ((d.flags >> 4) & 15u) > BFUSE_ACT_SILU) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": unknown activation");
+      if (act && (d.flags & BFUSE_FLAG_MUL) && !a[3]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": BFUSE_FLAG_MUL without the factor");
+      GemmActParams p;
       std::memset(&p, 0, sizeof(p));
       int rc = encode_map(ctx, &p.map_a, eb, a[0], s[3], s[1], s[0], bm);
       if (rc) return rc;
       rc = encode_map(ctx, &p.map_b, eb, a[1], s[3], s[2], s[0], bn);
       if (rc) return rc;
-      rc = encode_map(ctx, &p.map_out, eb, a[3], s[2], s[1], s[0], 32);
+      void *const out = a[act ? 4 : 3];
+      rc = encode_map(ctx, &p.map_out, eb, out, s[2], s[1], s[0], 32);
       if (rc) return rc;
+      if (act && a[3]) {
+        rc = encode_map(ctx, &p.map_other, eb, a[3], s[2], s[1], s[0], 32);
+        if (rc) return rc;
+        p.has_other = 1;
+      }
+      p.mul = act && (d.flags & BFUSE_FLAG_MUL) ? 1 : 0;
+      p.act = act ? (int)((d.flags >> 4) & 15u) : 0;
       p.bias = (const float *)a[2];
-      p.out = a[3];
+      p.out = out;
       p.batch = s[0], p.M = s[1], p.N = s[2], p.K = s[3];
       p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL);
       p.stages = std::min<int>(kUmmaMaxStages, (int)((k.smem - kUmmaHeaderBytes) / umma_stage_bytes(bn, bm)));
@@ -780,7 +945,13 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
 // epilogue can live with, stages it has now.  False for operators without a ring.
 bool ring_info(const KernelRec &k, int *header, int *stage_bytes, int *min_stages, int *stages) {
   const int *s = k.desc.shape;
-  if (k.desc.op == BFUSE_OP_GEMM_TF32 || k.desc.op == BFUSE_OP_GEMM_BF16) {
+  if (k.desc.op == BFUSE_OP_ATTENTION_BF16) {
+    *header = kUmmaHeaderBytes + attn_tile_bytes(s[5]), *stage_bytes = attn_tile_bytes(s[5]);
+    *min_stages = attention_min_stages(s[5], std::max(1, s[8]));
+    *stages = reinterpret_cast<const AttentionParams *>(k.params)->stages;
+    return true;
+  }
+  if (is_gemm_umma(k.desc.op)) {
     const int eb = k.desc.op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
     const int bm = s[6] > 0 ? s[6] : kUmmaBM;
     *header = kUmmaHeaderBytes, *stage_bytes = umma_stage_bytes(s[4], bm);
@@ -819,6 +990,7 @@ const void *params_with_stages(const KernelRec &k, int stages, unsigned char *sc
   std::memcpy(scratch, k.params, kParamsBytes);
   if (whole_planes(k)) reinterpret_cast<ConvUmmaParams *>(scratch)->st.slots = stages;
   else if (k.desc.op == BFUSE_OP_CONV2D_TF32) reinterpret_cast<ConvUmmaParams *>(scratch)->stages = stages;
+  else if (k.desc.op == BFUSE_OP_ATTENTION_BF16) reinterpret_cast<AttentionParams *>(scratch)->stages = stages;
   else reinterpret_cast<GemmUmmaParams *>(scratch)->stages = stages;
   return scratch;
 }
@@ -829,8 +1001,9 @@ int add_unsplit(bfuse_context *ctx, int reg, bool gathered, int *slot) {
   const KernelRec &orig = *ctx->kernels[reg];
   std::unique_ptr<KernelRec> alt(new KernelRec(orig));
   const bool conv = orig.desc.op == BFUSE_OP_CONV2D_TF32;
-  alt->desc.shape[conv ? 10 : 5] = 1;
-  if (!conv) alt->desc.shape[6] = 0;   // tile height: the runtime's choice for the unsplit form
+  const bool attention = orig.desc.op == BFUSE_OP_ATTENTION_BF16;
+  alt->desc.shape[conv ? 10 : attention ? 8 : 5] = 1;
+  if (!conv && !attention) alt->desc.shape[6] = 0;   // tile height: the runtime's choice for the unsplit form
   if (gathered) alt->desc.shape[9] = 0, alt->desc.shape[11] = 2;
   alt->desc.KernelName = nullptr;
   std::string err;
@@ -1128,7 +1301,8 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
   f->stages[0] = f->stages[1] = 0;
   // tensor-memory columns an operator's CTA allocates
   auto tmem_cols = [](const KernelRec &k) {
-    if (k.desc.op == BFUSE_OP_GEMM_TF32 || k.desc.op == BFUSE_OP_GEMM_BF16) return k.desc.shape[4] * std::max(1, k.desc.shape[6] / kUmmaBM);
+    if (is_gemm_umma(k.desc.op)) return k.desc.shape[4] * std::max(1, k.desc.shape[6] / kUmmaBM);
+    if (k.desc.op == BFUSE_OP_ATTENTION_BF16) return kAttnTmemCols;
     if (k.desc.op == BFUSE_OP_CONV2D_TF32 && (k.desc.shape[11] & 1)) return kConvTmemCols;   // staged: accumulator and operand stages
     return k.desc.op == BFUSE_OP_CONV2D_TF32 ? (k.desc.shape[9] > 0 ? k.desc.shape[9] : kConvBN) : 0;
   };
@@ -1206,7 +1380,7 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
   // 14 % slower by pattern (softmax of 1500 blocks beside 48 CTAs: zig-zag 13.9 -> 15.8 us, range split 17.5 -> 16.6).  Causal QK^T of 6 heads of 1024 tokens beside the softmax of 6 heads (9.6 and 9.1 us alone): 39.0 us,
   // 27.3 with the register-rich build, 21.2 with runs of 4; PV beside the softmax 31.6, 22.8, 18.2 (runs of 2; 20.0 with 4).
   // Smaller windows for the GEMM do not help: with four CTAs an SM in 64 registers QK^T || softmax takes 23-28 us.
-  auto memory_bound = [](const KernelRec &k) { return k.desc.op <= BFUSE_OP_ROPE_BF16; };
+  auto memory_bound = [](const KernelRec &k) { return k.desc.op <= BFUSE_OP_ROPE_BF16 || k.desc.op == BFUSE_OP_RESIDUAL_NORM_BF16; };
   const int row = memory_bound(*a) && tmem_cols(*b) ? 0 : memory_bound(*b) && tmem_cols(*a) ? 1 : -1;
   const bool row_rich = row >= 0 && by_smem <= pe.wide_min_blocks;
   if (row_rich && !thread_split && !t.queue) {
@@ -1687,7 +1861,7 @@ int bfuse_debug_gemm_timeline(bfuse_context *ctx, int kernel, long long *marks, 
   KernelRec *k = get_kernel(ctx, kernel);
   if (!k || !marks || n < MARK_COUNT) return fail(ctx, BFUSE_ERR_INVALID, "bad kernel handle or buffer shorter than 12 marks");
   const bool is_conv = k->desc.op == BFUSE_OP_CONV2D_TF32;
-  if (k->desc.op != BFUSE_OP_GEMM_TF32 && k->desc.op != BFUSE_OP_GEMM_BF16 && !is_conv)
+  if (!is_gemm_umma(k->desc.op) && !is_conv)
     return fail(ctx, BFUSE_ERR_UNSUPPORTED, "only the tcgen05 GEMM / conv bodies record a timeline");
   cudaSetDevice(ctx->device);
   long long *d = nullptr;
@@ -1801,6 +1975,7 @@ static int finish(bfuse_context *ctx, cudaStream_t s) {
   if (st) {
     cudaMemset(ctx->d_status, 0, sizeof(int));
     reset_queue_counters(ctx);
+    if (st == BFUSE_STATUS_BAD_OFFSETS) return fail(ctx, BFUSE_ERR_INVALID, "attention: sequence offsets fall or leave the tensors");
     char buf[64];
     snprintf(buf, sizeof(buf), "device status 0x%x: a bounded wait gave up", st);
     return fail(ctx, BFUSE_ERR_TIMEOUT, buf);

@@ -59,11 +59,45 @@ enum {
                               /* (staged wherever it can be), which writes 1, 2 or 3 back; a kernel          */
                               /* registered with 0 is gathered, and so is one whose 3 was written back and   */
                               /* that comes with the gathered form's GridDim or a window only that form fits */
-  BFUSE_OP_COUNT = 9
+  BFUSE_OP_GEMM_ACT_BF16 = 9, /* args: A, W, bias|NULL, other|NULL, out   shape: batch, M, N, K, tiling as GEMM_BF16;  */
+                              /* out = act(A W^T + bias) + other, or * other with BFUSE_FLAG_MUL; act: BFUSE_FLAG_ACT;  */
+                              /* A, W, other, out bf16 (other in out's shape; it may be out), bias fp32; accumulated,   */
+                              /* activated and added in fp32, rounded once                                              */
+  BFUSE_OP_RESIDUAL_NORM_BF16 = 10, /* args: x, block, gate|NULL, w|NULL, r|NULL, y|NULL   fparam: eps, scale           */
+                              /* shape: rows, cols (a multiple of 8, at most 8192), norms (a sum of BFUSE_NORM_*), rows */
+                              /* that share a row of the gate (0: all do);  with N(v) = v / sqrt(mean(v^2) + eps):      */
+                              /* b = block, or N(block) * w[after];  r = x + scale * gate * b;  y = N(r) * w[before].   */
+                              /* w holds a row of cols for each norm there is, in that order; y goes with the second    */
+                              /* norm, r may be left out beside it; r or y may be x or block                            */
+  BFUSE_OP_ATTENTION_BF16 = 11, /* args: q, k, v, cu_q, cu_kv|NULL, out   fparam: scale   flags: BFUSE_FLAG_CAUSAL      */
+                              /* shape: seqs, total_q, total_kv, heads, kv_heads, dim (a multiple of 8, at most 128),   */
+                              /* q token stride, k / v token stride (elements, multiples of 8; 0: dense), key slices    */
+                              /* per tile (1, 2, 4 or 8: a thread-block cluster joins them; 0: the runtime's choice).   */
+                              /* q [total_q, heads, dim], k and v [total_kv, kv_heads, dim], out [total_q, heads, dim]  */
+                              /* dense; query head h reads kv head h / (heads / kv_heads).  cu_q and cu_kv hold         */
+                              /* seqs + 1 rising token offsets (int32, DEVICE memory, read at every launch; NULL: cu_q): */
+                              /* sequence i has queries cu_q[i]..cu_q[i+1] and keys cu_kv[i]..cu_kv[i+1], any of them   */
+                              /* none; rows outside every sequence are left as they were.  Causal: the last query sees  */
+                              /* the last key, the one before all but it, and so on.  A query without keys gives zeros. */
+                              /* Keys and values outside a sequence may hold anything; inside one, a masked key may be  */
+                              /* NaN or infinite, a masked value must be finite.  Offsets that fall or leave the        */
+                              /* tensors: their sequence is left out and bfuse_read_status says BFUSE_STATUS_BAD_OFFSETS */
+  BFUSE_OP_COUNT = 12
 };
 
+/* a status word (bfuse_read_status) that no bounded wait left */
+#define BFUSE_STATUS_BAD_OFFSETS (-1)
+
+/* norms of BFUSE_OP_RESIDUAL_NORM_BF16: after the block, before the next one */
+enum { BFUSE_NORM_AFTER = 1, BFUSE_NORM_BEFORE = 2 };
+
+/* activations of BFUSE_OP_GEMM_ACT_BF16; GELU is x Phi(x), GELU_TANH its tanh form */
+enum { BFUSE_ACT_NONE = 0, BFUSE_ACT_RELU = 1, BFUSE_ACT_GELU = 2, BFUSE_ACT_GELU_TANH = 3, BFUSE_ACT_SILU = 4 };
+
 /* operator flags */
-#define BFUSE_FLAG_CAUSAL 1u /* GEMM: out[b,m,n] = -FLT_MAX where n > m */
+#define BFUSE_FLAG_CAUSAL 1u /* GEMM: out[b,m,n] = -FLT_MAX where n > m; attention: later keys are not seen */
+#define BFUSE_FLAG_MUL 2u    /* GEMM_ACT: the other operand multiplies instead of being added */
+#define BFUSE_FLAG_ACT(a) ((unsigned)(a) << 4) /* GEMM_ACT: BFUSE_ACT_* */
 /* Hint to bfuse_default_launch: n operators (1..4) will share the launch, so tile this one for 1/n of
  * the SMs; 1 = it runs alone.  Absent = 2, a pair.  Never changes results except through the k-slices. */
 #define BFUSE_FLAG_SHARE(n) ((unsigned)(n) << 8)
