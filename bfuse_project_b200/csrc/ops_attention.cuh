@@ -13,7 +13,9 @@
 // A tile is 128 rows of queries that share one key / value head: P = 128 / G consecutive positions of
 // one sequence times the G query heads of the group, so a single token of a grouped model fills G rows
 // and a prompt's tile reads each key once for the whole group.  BlockDim = (192, 1, 1): warps 0-3 own
-// the rows (thread = row = lane of tensor memory), warp 4 issues the TMA loads, warp 5 the MMAs.
+// the rows (thread = row = lane of tensor memory), warp 4 issues the TMA loads, warp 5 the MMAs.  (Eight
+// warps, two threads a row, are no faster: MUFU sets the pace of the exponentials either way, and the two
+// have to exchange their maxima in every block.)
 // GridDim = (slices * kv heads, tiles); the tiles are counted from the sequence offsets on the device
 // (`find_tile`), the host knows only their number at most: (total_q + seqs (P - 1)) / P.  The last
 // tile of a sequence, the one with the most keys under a causal mask, comes first.
@@ -23,19 +25,25 @@
 // do -- first every rank's (m, l) of every row, then its O scaled by 2^(m_rank - m) / l, summed in rank
 // order by the rank that owns the columns (deterministic).
 //
-// Tensor memory: S in columns 0-127, the bf16 p over its first 64, O in columns 128 up: 256 columns, so
-// two CTAs share an SM and one's MMAs run under the other's exponentials.
+// A tile of at most 16 rows (single tokens) would leave most of those exponentials to rows that are not
+// there.  It is multiplied the other way round: S^T = K Q^T and O^T += V^T p^T, keys (then dims) in the
+// lanes and the rows in 16 columns; a thread owns a key, p^T goes through shared memory, and S of the next
+// block is made while this one's exponentials are taken.
+//
+// Tensor memory: S in columns 0-127, O in columns 128 up, the bf16 p in 64 columns of its own behind O where
+// there is room (heads of up to 64 in 256 columns; 512 columns where only one CTA fits an SM anyway), else over S.
+// Two CTAs of 256 columns share an SM, and one's MMAs run under the other's exponentials.
 #pragma once
 
 #include "ops_umma.cuh"
 
 namespace bfuse {
 
-constexpr int kAttnThreads = 192;
+__host__ __device__ constexpr int attn_threads(int tiles) { return 128 * tiles + 64; }
 constexpr int kAttnRows = 128;     // query rows of a tile
 constexpr int kAttnKeys = 128;     // keys of a block
 constexpr int kAttnChunkBytes = 128 * 128;   // 128 rows x 64 bf16: what one TMA box holds
-constexpr int kAttnTmemCols = 256;
+constexpr int kAttnFewRows = 16;   // tiles of at most so many rows run transposed
 constexpr int kAttnMaxStages = 8;
 
 enum AttnStatus : int {
@@ -51,7 +59,7 @@ enum AttnStatus : int {
 
 __host__ __device__ constexpr int attn_chunks(int dim) { return dim <= 64 ? 1 : 2; }   // 64-element chunks of a head
 __host__ __device__ constexpr int attn_tile_bytes(int dim) { return attn_chunks(dim) * kAttnChunkBytes; }
-__host__ __device__ constexpr int attn_smem_bytes(int dim, int stages) { return kUmmaHeaderBytes + (1 + stages) * attn_tile_bytes(dim); }
+__host__ __device__ constexpr int attn_smem_bytes(int dim, int tiles, int stages) { return kUmmaHeaderBytes + (tiles + stages) * attn_tile_bytes(dim); }
 // what the slices of a tile exchange at the end: (m, l) per rank and row, and per 16 owned columns 8 KB of every rank
 __host__ __device__ constexpr int attn_join_bytes(int dim, int split) {
   return split > 1 ? split * kAttnRows * 8 + ((attn_chunks(dim) * 4 + split - 1) / split) * split * 16 * kAttnRows * 4 : 0;
@@ -66,6 +74,7 @@ struct AttentionParams {
   int seqs, total_q, total_kv, heads, kv_heads, dim;
   int group, positions;            // query heads per kv head; positions of a tile
   int causal, split, stages;
+  int tmem_cols, p_col;            // tensor memory: columns in all; first column of p, 0: over the scores
   float scale_log2;                // scale * log2(e), positive
 };
 
@@ -121,30 +130,47 @@ struct AttnTile {
   int keys;       // keys that any row of the tile may see
 };
 
-struct AttentionBf16 {
+// T tiles of one sequence and kv head per CTA: 1, or 2 that share every block of keys (four more warps; whole tiles only).
+template <int T>
+struct Attention {
   using Params = AttentionParams;
-  static constexpr int kMaxThreads = kAttnThreads;
-  static constexpr int kMinBlocks = 2;   // two CTAs an SM: 168 registers a thread
+  static constexpr int kMaxThreads = attn_threads(T);
+  static constexpr int kMinBlocks = T == 1 ? 2 : 1;   // two CTAs an SM: 168 registers a thread, 128 of them a row's scores
   static constexpr bool kMemoryBound = false;
   static constexpr bool kUsesTmem = true;
+  static constexpr int kProducer = 4 * T, kIssuer = kProducer + 1;   // warps
 
-  // Tile number t of the batch: sequence i has ceil(len_i / P) of them.  One warp; 256 sequences a round, 8 a lane,
+  // The window: [0, 1024) barriers, tensor-memory pointer and the tile; [1024, 2048) what the threads of a row exchange;
+  // then Q and the ring of `stages` K / V blocks in the order K0 V0 K1 V1 ...
+  struct Window {
+    // s_bar, pv_bar, o_bar, c_bar: one per tile, p_bar: two per tile (few rows: two s_bar and p_bar, by the parity of the block)
+    uint32_t full0, empty0, q_bar, s_bar, p_bar, pv_bar, o_bar, c_bar, stats_bar, join_bar;
+    uint32_t xch, q, ring;
+    int chunks, tile_bytes;
+  };
+  static constexpr int kBars = 2 * kAttnMaxStages + 15;
+
+  // Tile number t of the batch (T = 2: pair of tiles): sequence i has ceil(len_i / (T P)) of them.  One warp; 256 sequences a round, 8 a lane,
   // so that a batch of single tokens costs one trip to memory for its offsets and not one per 32 sequences.
   __device__ __forceinline__ static AttnTile find_tile(const Params &p, int t, int lane, int *status) {
+    const int positions = T * p.positions;
     AttnTile tile;
     tile.found = 0;
     int before = 0;   // tiles of the sequences before this round's
     for (int base = 0; base < p.seqs; base += 256) {
       const int s0 = base + lane * 8;
-      int cu[9], n[8], mine = 0;
+      int cu[9], kv[9], n[8], mine = 0;
 #pragma unroll
-      for (int i = 0; i < 9; ++i) cu[i] = s0 + i <= p.seqs ? __ldg(p.cu_q + s0 + i) : 0;
+      for (int i = 0; i < 9; ++i) {
+        cu[i] = s0 + i <= p.seqs ? __ldg(p.cu_q + s0 + i) : 0;
+        kv[i] = s0 + i <= p.seqs ? __ldg(p.cu_kv + s0 + i) : 0;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         n[i] = 0;
         if (s0 + i < p.seqs) {
           if (cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > p.total_q) atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS);
-          else n[i] = (cu[i + 1] - cu[i] + p.positions - 1) / p.positions;
+          else n[i] = (cu[i + 1] - cu[i] + positions - 1) / positions;
         }
         mine += n[i];
       }
@@ -165,22 +191,20 @@ struct AttentionBf16 {
             if (!done && t < at + n[i]) {
               done = true;
               const int qt = n[i] - 1 - (t - at);   // the last positions first
-              const int kv_a = __ldg(p.cu_kv + s0 + i), kv_b = __ldg(p.cu_kv + s0 + i + 1);
               const int q_len = cu[i + 1] - cu[i];
-              tile.found = kv_a >= 0 && kv_b >= kv_a && kv_b <= p.total_kv;
+              tile.found = kv[i] >= 0 && kv[i + 1] >= kv[i] && kv[i + 1] <= p.total_kv;
               if (!tile.found) atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS);
-              tile.q0 = cu[i] + qt * p.positions;
-              tile.npos = min(p.positions, q_len - qt * p.positions);
-              tile.kv0 = kv_a;
-              tile.kv_len = kv_b - kv_a;
-              tile.last0 = tile.kv_len - q_len + qt * p.positions;
+              tile.q0 = cu[i] + qt * positions;
+              tile.npos = min(positions, q_len - qt * positions);
+              tile.kv0 = kv[i];
+              tile.kv_len = kv[i + 1] - kv[i];
+              tile.last0 = tile.kv_len - q_len + qt * positions;
               tile.keys = p.causal ? max(0, min(tile.kv_len, tile.last0 + tile.npos)) : tile.kv_len;
             }
             at += n[i];
           }
         }
-        const unsigned who = __ballot_sync(0xffffffffu, here);
-        const int src = __ffs(who) - 1;
+        const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
         tile.found = __shfl_sync(0xffffffffu, tile.found, src);
         tile.q0 = __shfl_sync(0xffffffffu, tile.q0, src);
         tile.npos = __shfl_sync(0xffffffffu, tile.npos, src);
@@ -195,9 +219,32 @@ struct AttentionBf16 {
     return tile;
   }
 
-  __device__ __forceinline__ static void load_kv(const CUtensorMap *map, uint32_t dst, uint32_t bar, int chunks, int head, int token) {
-    mbar_expect_tx(bar, (uint32_t)chunks * kAttnChunkBytes);
-    for (int ch = 0; ch < chunks; ++ch) tma_load_3d(dst + ch * kAttnChunkBytes, map, bar, ch * 64, head, token);
+  // this slice's blocks of keys: first and count
+  __device__ __forceinline__ static void my_blocks(const AttnTile &t, int split, int slice, int &b0, int &n) {
+    const int nblocks = (t.keys + kAttnKeys - 1) / kAttnKeys, per = (nblocks + split - 1) / split;
+    b0 = min(nblocks, slice * per);
+    n = min(nblocks, b0 + per) - b0;
+  }
+  __device__ __forceinline__ static bool few_rows(const Params &p, const AttnTile &t) { return T == 1 && t.npos * p.group <= kAttnFewRows; }
+  // tile x of the CTA's, and its blocks of keys (those that some row of it may see come first in the CTA's n)
+  __device__ __forceinline__ static AttnTile sub_tile(const Params &p, const AttnTile &t, int x) {
+    if (T == 1) return t;
+    AttnTile s = t;
+    s.npos = max(0, min(p.positions, t.npos - x * p.positions));
+    s.q0 += x * p.positions;
+    s.last0 += x * p.positions;
+    s.keys = s.npos == 0 ? 0 : p.causal ? max(0, min(s.kv_len, s.last0 + s.npos)) : s.kv_len;
+    return s;
+  }
+  __device__ __forceinline__ static int sub_blocks(const AttnTile &s, int n) { return T == 1 ? n : (s.keys + kAttnKeys - 1) / kAttnKeys; }
+
+  // load i of the ring: K or V of block i / 2
+  __device__ __forceinline__ static void load(const Params &p, const Window &w, const AttnTile &t, int head, int b0, int i, uint32_t slot) {
+    const uint32_t bar = w.full0 + 8 * slot, dst = w.ring + slot * w.tile_bytes;
+    const int token = t.kv0 + (b0 + (i >> 1)) * kAttnKeys;
+    const CUtensorMap *map = i & 1 ? &p.map_v : &p.map_k;
+    mbar_expect_tx(bar, (uint32_t)w.tile_bytes);
+    for (int ch = 0; ch < w.chunks; ++ch) tma_load_3d(dst + ch * kAttnChunkBytes, map, bar, ch * 64, head, token);
   }
 
   // 16 finished columns of a row
@@ -208,54 +255,89 @@ struct AttentionBf16 {
         *reinterpret_cast<uint4 *>(row + col + 8 * j) = make_uint4(f2_to_bf16x2(v[8 * j], v[8 * j + 1]), f2_to_bf16x2(v[8 * j + 2], v[8 * j + 3]),
                                                                    f2_to_bf16x2(v[8 * j + 4], v[8 * j + 5]), f2_to_bf16x2(v[8 * j + 6], v[8 * j + 7]));
   }
+  // element 0 of a row of the tile in out
+  __device__ __forceinline__ static uint16_t *out_row(const Params &p, const AttnTile &t, int head, int row) {
+    const int pos = row / p.group;
+    return p.out + ((size_t)(t.q0 + pos) * p.heads + head * p.group + (row - pos * p.group)) * p.dim;
+  }
 
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
     const int warp = c.tid >> 5, lane = c.tid & 31;
-    const int quad = (threadIdx.x >> 5) & 3;   // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
     const int split = p.split, stages = p.stages;
     const int bx = c.block_x(), slice = bx % split, head = bx / split;
-    const int chunks = attn_chunks(p.dim), tile_bytes = chunks * kAttnChunkBytes;
-
-    // window: [0, 1024) barriers, tensor-memory pointer and the tile; from kUmmaHeaderBytes on Q, then the ring of
-    // `stages` K / V blocks in the order K0 V0 K1 V1 ...
-    uint64_t *bars = reinterpret_cast<uint64_t *>(c.smem);
-    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kAttnMaxStages, q_bar = empty0 + 8 * kAttnMaxStages;
-    const uint32_t s_bar = q_bar + 8, p_bar = q_bar + 16, o_bar = q_bar + 24, stats_bar = q_bar + 32, join_bar = q_bar + 40;
-    constexpr int kBars = 2 * kAttnMaxStages + 6;
+    Window w;
+    w.full0 = smem_u32(c.smem), w.empty0 = w.full0 + 8 * kAttnMaxStages, w.q_bar = w.empty0 + 8 * kAttnMaxStages;
+    w.s_bar = w.q_bar + 8, w.p_bar = w.q_bar + 24, w.pv_bar = w.q_bar + 56, w.o_bar = w.q_bar + 72, w.c_bar = w.q_bar + 88, w.stats_bar = w.q_bar + 104, w.join_bar = w.q_bar + 112;
+    w.xch = w.full0 + 1024, w.q = w.full0 + kUmmaHeaderBytes;
+    w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * kBars);
     AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 256);
-    const uint32_t q_smem = smem_u32(c.smem) + kUmmaHeaderBytes, ring = q_smem + tile_bytes;
 
-    if (warp == 5 && !c.tmem_given) {
-      tmem_alloc(smem_u32(tmem_slot), kAttnTmemCols);
+    if (warp == kIssuer && !c.tmem_given) {
+      tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
       if (!c.persistent) tmem_relinquish();
     }
-    c.dependency_wait();
-    if (warp == 4) {
+    int loaded = 0;
+    if (warp == kProducer) {
+      if (lane < stages) {
+        mbar_init(w.full0 + 8 * lane, 1);
+        mbar_init(w.empty0 + 8 * lane, 1);
+      }
+      if (lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_v) : "memory");
+      }
+      c.dependency_wait();
       const AttnTile t = find_tile(p, c.block_y(), lane, c.status);
-      const int active = t.found ? (t.npos * p.group + 31) >> 5 : 0;   // warps that own a row
+      const bool few = t.found && few_rows(p, t);
+      const int active = t.found ? (sub_tile(p, t, 0).npos * p.group + 31) >> 5 : 0;   // quarters of the (first) tile that hold a row
+      int b0 = 0, n = 0;
+      if (t.found) my_blocks(t, split, slice, b0, n);
       if (lane == 0) {
         *tile_slot = t;
-        for (int i = 0; i < stages; ++i) {
-          mbar_init(full0 + 8 * i, 1);
-          mbar_init(empty0 + 8 * i, 1);
+        mbar_init(w.q_bar, 1);
+        mbar_init(w.stats_bar, 1);
+        mbar_init(w.join_bar, 1);
+        for (int x = 0; x < 2; ++x) {
+          const int threads = few ? 128 : x == 0 || T == 1 ? active * 32 : t.found ? (sub_tile(p, t, x).npos * p.group + 31) & ~31 : 0;
+          mbar_init(w.s_bar + 8 * x, 1);
+          mbar_init(w.pv_bar + 8 * x, 1);
+          mbar_init(w.o_bar + 8 * x, 1);
+          mbar_init(w.c_bar + 8 * x, max(threads, 1));
+          mbar_init(w.p_bar + (T == 1 ? 8 : 16) * x, max(threads, 1));
+          if (T == 2) mbar_init(w.p_bar + 16 * x + 8, max(threads, 1));
         }
-        mbar_init(q_bar, 1);
-        mbar_init(s_bar, 1);
-        mbar_init(p_bar, active > 0 ? active * 32 : 1);
-        mbar_init(o_bar, 1);
-        mbar_init(stats_bar, 1);
-        mbar_init(join_bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      __syncwarp();
+      loaded = min(stages, 2 * n);
+      if (elect_one()) {
         if (split > 1 && t.found) {
-          // what this CTA will receive: (m, l) of every row from every rank, and the columns that it owns
-          int owned = 0;
-          for (int ch = slice; ch < chunks * 4; ch += split) ++owned;
-          mbar_expect_tx(stats_bar, (uint32_t)(split * active * 32 * 8));
-          if (owned) mbar_expect_tx(join_bar, (uint32_t)(owned * split * active * 32 * 64));
+          // what this CTA will receive: (m, l) of every row from every rank, and the columns (few rows: dims) that it owns
+          if (few) {
+            const int r = t.npos * p.group <= 8 ? 8 : kAttnFewRows;
+            mbar_expect_tx(w.stats_bar, (uint32_t)(split * r * 8));
+            mbar_expect_tx(w.join_bar, (uint32_t)(w.chunks * 64 * r * 4));
+          } else {
+            int owned = 0;
+            for (int ch = slice; ch < w.chunks * 4; ch += split) ++owned;
+            mbar_expect_tx(w.stats_bar, (uint32_t)(split * active * 32 * 8));
+            if (owned) mbar_expect_tx(w.join_bar, (uint32_t)(owned * split * active * 32 * 64));
+          }
+        }
+        if (n > 0) {   // the first round of the ring: every slot is free
+          const int tiles = T == 2 && t.npos > p.positions ? 2 : 1;
+          mbar_expect_tx(w.q_bar, (uint32_t)(tiles * w.chunks * p.group * p.positions * 128));
+          for (int x = 0; x < tiles; ++x)
+            for (int ch = 0; ch < w.chunks; ++ch)
+              tma_load_3d(w.q + x * w.tile_bytes + ch * kAttnChunkBytes, &p.map_q, w.q_bar, ch * 64, head * p.group, t.q0 + x * p.positions);
+          for (int i = 0; i < loaded; ++i) load(p, w, t, head, b0, i, (uint32_t)i);
         }
       }
       __syncwarp();
+    } else {
+      c.dependency_wait();
     }
     tc_fence_before();
     c.sync();
@@ -263,218 +345,320 @@ struct AttentionBf16 {
     const uint32_t tmem = c.tmem_given ? c.tmem_base : *reinterpret_cast<volatile uint32_t *>(tmem_slot);
     const AttnTile t = *tile_slot;
     if (t.found) {   // (the same for every CTA of a cluster)
-      const int nblocks = (t.keys + kAttnKeys - 1) / kAttnKeys, per = (nblocks + split - 1) / split;
-      const int b0 = min(nblocks, slice * per), n = min(nblocks, b0 + per) - b0;   // this slice's blocks of keys
-      if (warp == 4) produce(p, c, t, head, b0, n, full0, empty0, q_bar, q_smem, ring, chunks);
-      else if (warp == 5) multiply(p, c, n, tmem, full0, empty0, q_bar, s_bar, p_bar, o_bar, q_smem, ring, chunks);
-      const int rows = t.npos * p.group, row = quad * 32 + lane;
-      const bool mine = warp < 4 && quad * 32 < rows;   // this warp owns rows
-      float m = -INFINITY, l = 0.f;   // of this thread's row: the maximum the exponentials are taken against, and their sum
-      bool ok = true;
-      const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-      const int pos = row / p.group;
-      if (mine && n > 0) {
-        const int limit = row < rows ? (p.causal ? min(t.last0 + pos, t.kv_len - 1) : t.kv_len - 1) : -1;   // last key this row sees
-        ok = softmax(p, c, t, limit, b0, n, trow, full0, s_bar, p_bar, ring, chunks, m, l, active_threads(rows));
-        ok = warp_wait(o_bar, 0, c.status, ATTN_WAIT_OUT_TIMEOUT) && ok;
-        tc_fence_after();
-      }
-      uint16_t *out = p.out + ((size_t)(t.q0 + pos) * p.heads + head * p.group + (row - pos * p.group)) * p.dim;
-      if (split > 1) {
-        join(p, c, split, slice, n, chunks, rows, row, mine, ok, trow, q_smem, stats_bar, join_bar, m, l, out);
-      } else if (mine && ok) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-        for (int col = 0; col < p.dim; col += 32) {
-          uint32_t r[32];
-          if (n > 0) {
-            tmem_ld_32x32(trow + 128 + col, r);
-            tmem_ld_wait();
-          }
-          if (row < rows) {
-            float v[16];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = l == 0.f ? 0.f : __uint_as_float(r[16 * h + j]) * inv;   // a row without keys: zeros
-              store16(out, col + 16 * h, p.dim, v);
-            }
+      int b0, n;
+      my_blocks(t, split, slice, b0, n);
+      const bool few = few_rows(p, t);
+      if (warp == kProducer) {
+        if (n > 0 && elect_one()) {
+          uint32_t s = loaded == stages ? 0 : (uint32_t)loaded, ph = 0;
+          for (int i = loaded; i < 2 * n; ++i) {
+            if (!mbar_wait(w.empty0 + 8 * s, ph, c.status, ATTN_WAIT_SLOT_TIMEOUT)) break;
+            load(p, w, t, head, b0, i, s);
+            if (++s == (uint32_t)stages) s = 0, ph ^= 1;
           }
         }
+        __syncwarp();
+      } else if (warp == kIssuer) {
+        if (n > 0 && elect_one()) {
+          bool ok = mbar_wait(w.q_bar, 0, c.status, ATTN_WAIT_Q_TIMEOUT);
+          if (ok) ok = few ? multiply_few(p, c, w, n, tmem) : multiply(p, c, w, t, n, tmem);
+          if (T == 1) umma_commit(w.o_bar);
+          // the releases of the slots' last uses are asynchronous: none may be in flight when the barriers go
+          for (int i = max(0, 2 * n - stages); i < 2 * n && ok; ++i)
+            ok = mbar_wait(w.empty0 + 8 * (i % stages), (i / stages) & 1, c.status, ATTN_WAIT_SLOT_TIMEOUT);
+          for (int x = 0; x < T && ok; ++x) {
+            const int nx = sub_blocks(sub_tile(p, t, x), n);
+            if (nx > 0 && (few || p.p_col)) ok = mbar_wait(w.pv_bar + 8 * x, (nx - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+            if (nx > 0 && ok) ok = mbar_wait(w.o_bar + 8 * x, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          }
+        }
+        __syncwarp();
+      }
+      if constexpr (T == 2) {
+        const int x = warp >> 2;   // (the loading and issuing warps: 2, no tile)
+        if (x < T) {
+          const AttnTile s = sub_tile(p, t, x);
+          tile(p, c, w, s, head, 1, 0, 0, sub_blocks(s, n), tmem, x);
+        }
+      } else if (few) {
+        if (t.npos * p.group <= 8) few_tile<8>(p, c, w, t, head, split, slice, b0, n, tmem);
+        else few_tile<16>(p, c, w, t, head, split, slice, b0, n, tmem);
+      } else {
+        tile(p, c, w, t, head, split, slice, b0, n, tmem, 0);
       }
     }
     __syncwarp();
     tc_fence_before();
     c.sync();
-    if (warp == 5 && !c.tmem_given) tmem_dealloc(tmem, kAttnTmemCols);
+    if (warp == kIssuer && !c.tmem_given) tmem_dealloc(tmem, p.tmem_cols);
     if (c.persistent && c.tid < kBars) {   // the next tile of a persistent CTA initialises them again
       const int s = c.tid < kAttnMaxStages ? c.tid : c.tid - kAttnMaxStages;
-      if (c.tid >= 2 * kAttnMaxStages || s < stages) mbar_inval(full0 + 8 * c.tid);
+      if (c.tid >= 2 * kAttnMaxStages || s < stages) mbar_inval(w.full0 + 8 * c.tid);
     }
   }
 
-  __device__ __forceinline__ static int active_threads(int rows) { return min(128, (rows + 31) & ~31); }
+  // V as an operand whose rows are keys ("MN-major"): its 64-column chunks lie `chunk_step` bytes apart (leading offset),
+  // groups of 8 keys 1024 bytes (stride offset), 16 keys -- one instruction -- 2048
+  __device__ __forceinline__ static uint32_t v_desc(uint32_t addr, uint32_t chunk_step) { return ((addr >> 4) & 0x3fffu) | ((chunk_step >> 4) << 16); }
+  __device__ __forceinline__ static uint32_t k_major_desc(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
 
-  __device__ __forceinline__ static void produce(const Params &p, const TileCtx &c, const AttnTile &t, int head, int b0, int n, uint32_t full0,
-                                                 uint32_t empty0, uint32_t q_bar, uint32_t q_smem, uint32_t ring, int chunks) {
-    if (n > 0 && elect_one()) {
-      const int tile_bytes = chunks * kAttnChunkBytes;
-      mbar_expect_tx(q_bar, (uint32_t)(chunks * p.group * p.positions * 128));
-      for (int ch = 0; ch < chunks; ++ch) tma_load_3d(q_smem + ch * kAttnChunkBytes, &p.map_q, q_bar, ch * 64, head * p.group, t.q0);
-      uint32_t s = 0, ph = 1;   // (a slot's first use waits for nothing: parity 1 of a fresh barrier)
-      for (int i = 0; i < 2 * n; ++i) {
-        if (!mbar_wait(empty0 + 8 * s, ph, c.status, ATTN_WAIT_SLOT_TIMEOUT)) break;
-        load_kv(i & 1 ? &p.map_v : &p.map_k, ring + s * tile_bytes, full0 + 8 * s, chunks, head, t.kv0 + (b0 + (i >> 1)) * kAttnKeys);
-        if (++s == (uint32_t)p.stages) s = 0, ph ^= 1;
-      }
+  // ---- whole tiles: rows in the lanes ----
+
+  // A slot of the ring and the phase its barrier is in, carried along: loads are `step` apart (divisions would idle the tensor pipe).
+  struct RingAt {
+    uint32_t slot, phase;
+    __device__ __forceinline__ void advance(uint32_t step, uint32_t stages) {   // step <= stages
+      slot += step;
+      if (slot >= stages) slot -= stages, phase ^= 1;
     }
-    __syncwarp();
-  }
+  };
 
-  __device__ __forceinline__ static void multiply(const Params &p, const TileCtx &c, int n, uint32_t tmem, uint32_t full0, uint32_t empty0,
-                                                  uint32_t q_bar, uint32_t s_bar, uint32_t p_bar, uint32_t o_bar, uint32_t q_smem, uint32_t ring,
-                                                  int chunks) {
-    if (n > 0 && elect_one()) {
-      const uint32_t idesc_s = umma_idesc(1, kAttnKeys), idesc_o = umma_idesc(1, chunks * 64) | (1u << 16);   // V: keys are its rows ("MN-major")
-      const uint32_t tile16 = (uint32_t)(chunks * kAttnChunkBytes) >> 4;
-      const uint32_t q_lo = ((q_smem >> 4) & 0x3fffu) | (1u << 16), ring_lo = (ring >> 4) & 0x3fffu;
-      const int ksteps = (p.dim + 15) >> 4;   // 16 dims a step (the TMA filled up what dim does not have)
-      uint32_t s = 0, ph = 0;
-      bool ok = mbar_wait(q_bar, 0, c.status, ATTN_WAIT_Q_TIMEOUT);
-      for (int j = 0; j < n && ok; ++j) {
-        // S = Q K^T.  It may overwrite the p of block j - 1: the MMAs of one CTA run in the order they are issued
-        ok = mbar_wait(full0 + 8 * s, ph, c.status, ATTN_WAIT_KV_TIMEOUT);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t k_lo = (ring_lo + s * tile16) | (1u << 16);
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (uint32_t)(k >> 2) * (kAttnChunkBytes >> 4) + 2 * (k & 3);
-          umma_ss<1>(tmem, q_lo + off, k_lo + off, idesc_s, k > 0);
-        }
-        umma_commit(empty0 + 8 * s);
-        umma_commit(s_bar);
-        if (++s == (uint32_t)p.stages) s = 0, ph ^= 1;
-        // O += p V
-        ok = mbar_wait(p_bar, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT) && mbar_wait(full0 + 8 * s, ph, c.status, ATTN_WAIT_KV_TIMEOUT);
-        if (!ok) break;
-        tc_fence_after();
-        // 64-column chunks of V lie one box apart (leading offset), groups of 8 keys 1024 bytes (stride offset)
-        const uint32_t v_lo = (ring_lo + s * tile16) | ((uint32_t)(kAttnChunkBytes >> 4) << 16);
+  // S = Q K^T of tile x and the block of keys at k; `wait`: nobody has waited for them yet, `last`: no other tile reads them after it
+  __device__ __forceinline__ static bool scores(const Params &p, const TileCtx &c, const Window &w, const RingAt &k, uint32_t tmem, int x, bool wait, bool last) {
+    const uint32_t idesc = umma_idesc(1, kAttnKeys), q_lo = k_major_desc(w.q + x * w.tile_bytes);
+    const int ksteps = (p.dim + 15) >> 4;   // 16 dims a step (the TMA filled up what dim does not have)
+    if (wait) {
+      if (!mbar_wait(w.full0 + 8 * k.slot, k.phase, c.status, ATTN_WAIT_KV_TIMEOUT)) return false;
+      tc_fence_after();
+    }
+    const uint32_t k_lo = k_major_desc(w.ring + k.slot * w.tile_bytes);
 #pragma unroll
-        for (int k = 0; k < kAttnKeys / 16; ++k) umma_ts_bf16(tmem + 128, tmem + 8 * k, v_lo + 128 * k, idesc_o, j > 0 || k > 0);
-        umma_commit(empty0 + 8 * s);
-        if (++s == (uint32_t)p.stages) s = 0, ph ^= 1;
-      }
-      umma_commit(o_bar);
-      // the slot releases of the last uses are asynchronous: none may be in flight when the barriers go
-      const int uses = 2 * n;
-      for (int i = max(0, uses - p.stages); i < uses && ok; ++i)
-        ok = mbar_wait(empty0 + 8 * (i % p.stages), (i / p.stages) & 1, c.status, ATTN_WAIT_SLOT_TIMEOUT);
-      if (ok) mbar_wait(o_bar, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t off = (uint32_t)(i >> 2) * (kAttnChunkBytes >> 4) + 2 * (i & 3);
+      if (i < ksteps) umma_ss<1>(tmem + 256u * x, q_lo + off, k_lo + off, idesc, i > 0);
     }
-    __syncwarp();
+    if (last) umma_commit(w.empty0 + 8 * k.slot);
+    umma_commit(w.s_bar + 8 * x);
+    return true;
+  }
+
+  // Where p has columns of its own (p_col), S of block j + 1 is made as soon as the threads have S of block j in their
+  // registers, under its exponentials; else after p V of block j, since the MMAs of one CTA run in the order they are issued.
+  // p V starts with the 64 keys whose p comes first.  Two tiles take turns, one's MMAs under the other's exponentials.
+  __device__ __forceinline__ static bool multiply(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int n, uint32_t tmem) {
+    const uint32_t idesc = umma_idesc(1, w.chunks * 64) | (1u << 16), stages = (uint32_t)p.stages;
+    int nx[2] = {n, 0};
+    if (T == 2) nx[0] = sub_blocks(sub_tile(p, t, 0), n), nx[1] = sub_blocks(sub_tile(p, t, 1), n);
+    RingAt k{0, 0}, v{1, 0};
+    // block j is read by tile 0, if that has so many, and then by tile 1: the first waits for it, the last gives it up
+    auto first = [&](int j, int x) { return T == 1 || x == 0 || j >= nx[0]; };
+    auto last = [&](int j, int x) { return T == 1 || x == 1 || j >= nx[1]; };
+    for (int x = 0; x < T; ++x)
+      if (nx[x] > 0 && !scores(p, c, w, k, tmem, x, first(0, x), last(0, x))) return false;
+    k.advance(2, stages);
+    for (int j = 0; j < n; ++j) {
+      const uint32_t v_lo = v_desc(w.ring + v.slot * w.tile_bytes, kAttnChunkBytes);
+#pragma unroll
+      for (int x = 0; x < T; ++x) {
+        if (T == 2 && j >= nx[x]) continue;
+        const bool more = j + 1 < nx[x];
+        if (p.p_col && more) {
+          if (!mbar_wait(w.c_bar + 8 * x, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
+          tc_fence_after();
+          if (!scores(p, c, w, k, tmem, x, first(j + 1, x), last(j + 1, x))) return false;
+        }
+        if (first(j, x) && !mbar_wait(w.full0 + 8 * v.slot, v.phase, c.status, ATTN_WAIT_KV_TIMEOUT)) return false;
+        const uint32_t pt = tmem + 256u * x + (uint32_t)p.p_col;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!mbar_wait(w.p_bar + 16 * x + 8 * part, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t step = (uint32_t)(4 * part + i);   // of 16 keys
+            umma_ts_bf16(tmem + 256u * x + 128, pt + 8 * step, v_lo + 128 * step, idesc, j > 0 || part + i > 0);
+          }
+        }
+        if (last(j, x)) umma_commit(w.empty0 + 8 * v.slot);
+        if (p.p_col) umma_commit(w.pv_bar + 8 * x);
+        else if (more && !scores(p, c, w, k, tmem, x, first(j + 1, x), last(j + 1, x))) return false;
+        if (T == 2 && !more) umma_commit(w.o_bar + 8 * x);
+      }
+      v.advance(2, stages);
+      k.advance(2, stages);
+    }
+    return true;
   }
 
   // (a whole warp gives up or goes on: what follows are warp-wide tensor-memory instructions)
   __device__ __forceinline__ static bool warp_wait(uint32_t bar, uint32_t parity, int *status, int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
   }
+  __device__ __forceinline__ static float lds_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+  }
 
-  // The online softmax of one row over this slice's blocks.  False: a wait gave up.
-  __device__ __forceinline__ static bool softmax(const Params &p, const TileCtx &c, const AttnTile &t, int limit, int b0, int n, uint32_t trow,
-                                                 uint32_t full0, uint32_t s_bar, uint32_t p_bar, uint32_t ring, int chunks, float &m_out, float &l_out,
-                                                 int threads) {
-    const float sc = p.scale_log2;
-    float m = -INFINITY, l = 0.f;
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int key0 = (b0 + j) * kAttnKeys;
-      if (!warp_wait(s_bar, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT)) return false;
-      tc_fence_after();
-      const int seen = limit - key0;   // columns 0..seen of this block count
-      const bool masked = __any_sync(0xffffffffu, seen < kAttnKeys - 1);
-      float mx = m;
+  // Two values at a time: the packed fp32 instructions do two lanes' worth in one issue slot.
+  __device__ __forceinline__ static float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+  }
+  __device__ __forceinline__ static float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+  }
+
+  // Values past the end of the sequence are the next one's, or whatever the buffer holds: p is 0 there, but 0 * NaN is not,
+  // so those rows of V become zeros.  `first` of `threads` threads; the block's V is load 2 j + 1 of the ring.
+  __device__ __forceinline__ static bool clear_tail(const Params &p, const TileCtx &c, const Window &w, int j, int have, int first, int threads) {
+    const int i = 2 * j + 1, s = i % p.stages;
+    const bool ok = warp_wait(w.full0 + 8 * s, (i / p.stages) & 1, c.status, ATTN_WAIT_KV_TIMEOUT);
+    const uint32_t v = w.ring + s * w.tile_bytes;
+    if (ok)
+      for (int ch = 0; ch < w.chunks; ++ch)
+        for (int k = first; k < (kAttnKeys - have) * 8; k += threads) st_shared_u4(v + ch * kAttnChunkBytes + have * 128 + k * 16, 0, 0, 0, 0);
+    fence_async_smem();
+    return ok;
+  }
+
+  // the largest of three
+  __device__ __forceinline__ static float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+  }
+  // The 128 scores of a row: the largest (with m), then 32 of their exponentials as bf16 into tensor memory
+  template <bool MASKED>
+  __device__ __forceinline__ static float largest(uint32_t (&r)[4][32], int seen, float m) {
+    float mx[4] = {m, m, m, m};
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t r[32];
-        tmem_ld_32x32(trow + 32 * h, r);
-        tmem_ld_wait();
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (masked && 32 * h + i > seen) ? -INFINITY : __uint_as_float(r[i]));
+      for (int i = 0; i < 32; i += 2) {
+        if (MASKED && 32 * g + i > seen) r[g][i] = __float_as_uint(-INFINITY);
+        if (MASKED && 32 * g + i + 1 > seen) r[g][i + 1] = __float_as_uint(-INFINITY);
+        mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[g][i]), __uint_as_float(r[g][i + 1]));
       }
-      // O follows a larger maximum only when that grew by more than 2^8: p stays below 2^8 and the sums in fp32 lose
-      // nothing, and O mostly stays where it is.  (s_bar stands for every MMA before it, so block j - 1 is in O.)
-      if (__any_sync(0xffffffffu, (mx - m) * sc > 8.f)) {
-        const float f = mx == -INFINITY ? 1.f : ex2((m - mx) * sc);
-        m = mx;
-        l *= f;
-        if (j > 0) {
-#pragma unroll 1
-          for (int col = 0; col < chunks * 64; col += 16) {
-            uint32_t r[16];
-            tmem_ld_32x16(trow + 128 + col, r);
-            tmem_ld_wait();
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  }
+  __device__ __forceinline__ static void exponentials(uint32_t p_tmem, const uint32_t (&r)[32], float sc, float mc, float2 &sum) {
+    const float2 sc2 = make_float2(sc, sc), mc2 = make_float2(-mc, -mc);
+    uint32_t q[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-            tmem_st_32x16(trow + 128 + col, r);
+    for (int i = 0; i < 16; ++i) {
+      float2 a = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, mc2);
+      a.x = ex2(a.x), a.y = ex2(a.y);
+      sum = add2(sum, a);
+      q[i] = f2_to_bf16x2(a.x, a.y);   // the second product takes bf16: half a step of p, as of the output
+    }
+    tmem_st_32x16(p_tmem, q);
+  }
+
+  __device__ __forceinline__ static void tile(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice,
+                                              int b0, int n, uint32_t tmem_base, int x) {
+    const uint32_t tmem = tmem_base + 256u * x;
+    const int warp = c.tid >> 5, lane = c.tid & 31;
+    const int quad = (threadIdx.x >> 5) & 3;   // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
+    const int rows = t.npos * p.group, row = quad * 32 + lane, active = (rows + 31) >> 5;
+    const bool mine = warp < kProducer && quad < active;   // this warp owns rows
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
+    float m = -INFINITY, l = 0.f;   // the maximum the exponentials are taken against, and their sum
+    bool ok = true;
+    if (mine && n > 0) {
+      const int limit = row < rows ? (p.causal ? min(t.last0 + row / p.group, t.kv_len - 1) : t.kv_len - 1) : -1;   // last key this row sees
+      const float sc = p.scale_log2;
+#pragma unroll 1
+      for (int j = 0; j < n && ok; ++j) {
+        const int key0 = (b0 + j) * kAttnKeys;
+        ok = warp_wait(w.s_bar + 8 * x, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) tmem_ld_32x32(trow + 32 * g, r[g]);
+        tmem_ld_wait();
+        if (p.p_col) {
+          tc_fence_before();
+          mbar_arrive(w.c_bar + 8 * x);   // S may be overwritten
+        }
+        const int seen = limit - key0;   // columns 0..seen of this block count
+        const bool masked = __any_sync(0xffffffffu, seen < kAttnKeys - 1);
+        const float mx = masked ? largest<true>(r, seen, m) : largest<false>(r, seen, m);
+        if (p.p_col && j > 0) {   // p's columns are free, and O is whole, once p V of block j - 1 is done
+          ok = warp_wait(w.pv_bar + 8 * x, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          tc_fence_after();
+        }
+        // O follows a larger maximum only when that grew by more than 2^8: p stays below 2^8 and the sums in fp32 lose
+        // nothing, and O mostly stays where it is.  (Without p_col s_bar stands for every MMA before it: block j - 1 is in O.)
+        if (__any_sync(0xffffffffu, (mx - m) * sc > 8.f)) {
+          const float f = mx == -INFINITY ? 1.f : ex2((m - mx) * sc);
+          m = mx;
+          l *= f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int col = 0; col < w.chunks * 64; col += 16) {
+              uint32_t o[16];
+              tmem_ld_32x16(trow + 128 + col, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st_32x16(trow + 128 + col, o);
+            }
+          }
+        }
+        const int have = t.kv_len - key0;
+        if (have < kAttnKeys && ok) ok = clear_tail(p, c, w, j, have, row, active * 32);
+        const float mc = m == -INFINITY ? 0.f : m * sc;
+        const uint32_t p_tmem = trow + (uint32_t)p.p_col;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          exponentials(p_tmem + 16 * g, r[g], sc, mc, sum);
+          if (g & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(w.p_bar + 16 * x + 8 * (g >> 1));
+          }
+        }
+        l += sum.x + sum.y;
+      }
+      if (ok) ok = warp_wait(w.o_bar + 8 * x, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+      tc_fence_after();
+    }
+    if (T == 1 && split > 1) {
+      join(p, c, w, t, head, split, slice, n, rows, row, mine, ok, trow, m, l);
+    } else if (mine && ok) {
+      uint16_t *out = out_row(p, t, head, row);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int col = 0; col < p.dim; col += 32) {
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld_32x32(trow + 128 + col, r);
+          tmem_ld_wait();
+        }
+        if (row < rows) {
+          float v[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = l == 0.f ? 0.f : __uint_as_float(r[16 * h + j]) * inv;   // a row without keys: zeros
+            store16(out, col + 16 * h, p.dim, v);
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.f : m * sc;
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t r[32], q[16];
-        tmem_ld_32x32(trow + 32 * h, r);
-        tmem_ld_wait();
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a = __uint_as_float(r[2 * i]), b = __uint_as_float(r[2 * i + 1]);
-          if (masked && 32 * h + 2 * i > seen) a = -INFINITY;
-          if (masked && 32 * h + 2 * i + 1 > seen) b = -INFINITY;
-          a = ex2(fmaf(a, sc, -mc)), b = ex2(fmaf(b, sc, -mc));
-          sum += a + b;
-          q[i] = f2_to_bf16x2(a, b);   // the second product takes bf16: half a step of p, as of the output
-        }
-        l += sum;
-        tmem_st_32x16(trow + 16 * h, q);
-      }
-      // Past the end of the sequence lie the next one's values, or whatever the buffer holds: p is 0 there, but
-      // 0 * NaN is not, so those rows of V become zeros
-      const int have = t.kv_len - key0;
-      bool ok = true;
-      if (have < kAttnKeys) {
-        const int i = 2 * j + 1, s = i % p.stages;
-        ok = warp_wait(full0 + 8 * s, (i / p.stages) & 1, c.status, ATTN_WAIT_KV_TIMEOUT);
-        const uint32_t v = ring + s * chunks * kAttnChunkBytes;
-        const int vecs = (kAttnKeys - have) * 8;   // 16-byte pieces per chunk
-        const int quad = (threadIdx.x >> 5) & 3, first = quad * 32 + (c.tid & 31);
-        if (ok)
-          for (int ch = 0; ch < chunks; ++ch)
-            for (int k = first; k < vecs; k += threads) st_shared_u4(v + ch * kAttnChunkBytes + have * 128 + k * 16, 0, 0, 0, 0);
-        fence_async_smem();
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(p_bar);
-      if (!ok) return false;
     }
-    m_out = m, l_out = l;
-    return true;
   }
 
   // The slices of a tile become one result (all threads of every CTA of the cluster).
-  __device__ __forceinline__ static void join(const Params &p, const TileCtx &c, int split, int slice, int n, int chunks, int rows, int row, bool mine,
-                                              bool ok, uint32_t trow, uint32_t area, uint32_t stats_bar, uint32_t join_bar, float m, float l,
-                                              uint16_t *out) {
-    // every rank's MMAs are done: Q and the ring are free everywhere
-    cluster_sync_all();
+  __device__ __forceinline__ static void join(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice, int n,
+                                              int rows, int row, bool mine, bool ok, uint32_t trow, float m, float l) {
+    cluster_sync_all();   // every rank's MMAs are done: Q and the ring are free everywhere
     if (!mine) return;
     const float mlog = m * p.scale_log2;   // in powers of two
-    const uint32_t recv = area + (uint32_t)(split * kAttnRows * 8);
+    const uint32_t area = w.q, recv = area + (uint32_t)(split * kAttnRows * 8);
     for (int r = 0; r < split; ++r)
-      st_async_f2(peer_smem(area + (uint32_t)(slice * kAttnRows + row) * 8, r), peer_smem(stats_bar, r), mlog, l);
-    if (!warp_wait(stats_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT)) ok = false;
+      st_async_f2(peer_smem(area + (uint32_t)(slice * kAttnRows + row) * 8, r), peer_smem(w.stats_bar, r), mlog, l);
+    if (!warp_wait(w.stats_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT)) ok = false;
     float top = -INFINITY, sum = 0.f;
     for (int r = 0; r < split; ++r) top = fmaxf(top, ld_shared_f2(area + (uint32_t)(r * kAttnRows + row) * 8).x);
     if (top == -INFINITY) top = 0.f;
@@ -483,7 +667,7 @@ struct AttentionBf16 {
       sum += s.y * ex2(s.x - top);
     }
     const float f = l == 0.f ? 0.f : ex2(mlog - top) / sum;
-    const int pieces = chunks * 4;   // of 16 columns
+    const int pieces = w.chunks * 4;   // of 16 columns
 #pragma unroll 1
     for (int ch = 0; ch < pieces; ++ch) {
       uint32_t r[16];
@@ -494,28 +678,263 @@ struct AttentionBf16 {
 #pragma unroll
       for (int i = 0; i < 16; ++i) r[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(r[i]) * f);
       const uint32_t slot = recv + (uint32_t)((ch / split) * split + slice) * (16 * kAttnRows * 4);
-      const uint32_t dst = peer_smem(slot + (uint32_t)row * 16, ch % split), bar = peer_smem(join_bar, ch % split);
+      const uint32_t dst = peer_smem(slot + (uint32_t)row * 16, ch % split), bar = peer_smem(w.join_bar, ch % split);
 #pragma unroll
       for (int i = 0; i < 4; ++i) st_async_u4(dst + (uint32_t)(i * kAttnRows * 16), bar, r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
     }
     if (slice >= pieces) return;   // owns no columns
-    if (!warp_wait(join_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT) || !ok || row >= rows) return;
+    if (!warp_wait(w.join_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT) || !ok || row >= rows) return;
+    uint16_t *out = out_row(p, t, head, row);
 #pragma unroll 1
     for (int ch = slice; ch < pieces; ch += split) {
       float v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      for (int k = 0; k < 16; ++k) v[k] = 0.f;
       for (int r = 0; r < split; ++r) {   // rank order: the sum is deterministic
         const uint32_t src = recv + (uint32_t)((ch / split) * split + r) * (16 * kAttnRows * 4) + (uint32_t)row * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 a = ld_shared_f4(src + (uint32_t)(i * kAttnRows * 16));
-          v[4 * i] += a.x, v[4 * i + 1] += a.y, v[4 * i + 2] += a.z, v[4 * i + 3] += a.w;
+        for (int k = 0; k < 4; ++k) {
+          const float4 a = ld_shared_f4(src + (uint32_t)(k * kAttnRows * 16));
+          v[4 * k] += a.x, v[4 * k + 1] += a.y, v[4 * k + 2] += a.z, v[4 * k + 3] += a.w;
         }
       }
       store16(out, ch * 16, p.dim, v);
     }
   }
+
+  // ---- tiles of few rows: keys, then dims, in the lanes ----
+
+  // p^T of a block: 16 rows x 128 keys bf16, K-major in two 64-key chunks; two of them lie over the rows of the Q tile that a
+  // tile of few rows does not have
+  __device__ __forceinline__ static uint32_t pt_smem(const Window &w, int j) { return w.q + 2048u + (uint32_t)(j & 1) * 4096u; }
+
+  // S^T of block j + 1 = K Q^T goes into the other of two buffers while the threads work on block j (block j - 1 is done with
+  // it), then O^T += V^T p^T of block j.  The ring's loads are used in the order K0 K1 V0 K2 V1 ...
+  __device__ __forceinline__ static bool multiply_few(const Params &p, const TileCtx &c, const Window &w, int n, uint32_t tmem) {
+    const uint32_t idesc_s = umma_idesc(1, kAttnFewRows), idesc_o = idesc_s | (1u << 15), stages = (uint32_t)p.stages;   // V transposed
+    const uint32_t q_lo = k_major_desc(w.q), chunk_step = w.chunks == 2 ? kAttnChunkBytes : 0;   // (a head of one chunk fills 64 lanes, the others get it again)
+    const int ksteps = (p.dim + 15) >> 4;
+    RingAt k{0, 0}, v{1, 0};
+    for (int j = -1; j < n; ++j) {
+      if (j + 1 < n) {
+        if (!mbar_wait(w.full0 + 8 * k.slot, k.phase, c.status, ATTN_WAIT_KV_TIMEOUT)) return false;
+        tc_fence_after();
+        const uint32_t k_lo = k_major_desc(w.ring + k.slot * w.tile_bytes);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t off = (uint32_t)(i >> 2) * (kAttnChunkBytes >> 4) + 2 * (i & 3);
+          if (i < ksteps) umma_ss<1>(tmem + (uint32_t)((j + 1) & 1) * kAttnFewRows, k_lo + off, q_lo + off, idesc_s, i > 0);
+        }
+        umma_commit(w.empty0 + 8 * k.slot);
+        umma_commit(w.s_bar + 8 * ((j + 1) & 1));
+        k.advance(2, stages);
+      }
+      if (j < 0) continue;
+      // (the next block's p may be there before this wait is: a barrier for each of the two)
+      if (!mbar_wait(w.full0 + 8 * v.slot, v.phase, c.status, ATTN_WAIT_KV_TIMEOUT) ||
+          !mbar_wait(w.p_bar + 8 * (j & 1), (j >> 1) & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT))
+        return false;
+      tc_fence_after();
+      const uint32_t v_lo = v_desc(w.ring + v.slot * w.tile_bytes, chunk_step), pt_lo = k_major_desc(pt_smem(w, j));
+#pragma unroll
+      for (int i = 0; i < kAttnKeys / 16; ++i)
+        umma_ss<1>(tmem + 128, v_lo + 128 * i, pt_lo + (uint32_t)(i >> 2) * 128 + 2 * (i & 3), idesc_o, j > 0 || i > 0);
+      umma_commit(w.empty0 + 8 * v.slot);
+      umma_commit(w.pv_bar);
+      v.advance(2, stages);
+    }
+    return true;
+  }
+
+  // the four warps that own the lanes (barrier 9 or 10)
+  __device__ __forceinline__ static void quads_sync(const TileCtx &c) { asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory"); }
+  __device__ __forceinline__ static bool quads_any(const TileCtx &c, bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)x), "r"(c.bar_id + 8)
+        : "memory");
+    return any != 0;
+  }
+  // over the 128 lanes, for each of R values; everyone gets it
+  template <class Op, int R>
+  __device__ __forceinline__ static void quads_reduce(const TileCtx &c, const Window &w, int quad, int lane, float (&v)[R]) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = Op::apply(v[i], __shfl_xor_sync(0xffffffffu, v[i], off));
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i)
+        st_shared_u4(w.xch + (uint32_t)(quad * 64 + i * 16), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                     __float_as_uint(v[4 * i + 3]));
+    quads_sync(c);
+#pragma unroll
+    for (int i = 0; i < R / 4; ++i) {
+      float4 a = ld_shared_f4(w.xch + (uint32_t)(i * 16));
+#pragma unroll
+      for (int k = 1; k < 4; ++k) {
+        const float4 b = ld_shared_f4(w.xch + (uint32_t)(k * 64 + i * 16));
+        a.x = Op::apply(a.x, b.x), a.y = Op::apply(a.y, b.y), a.z = Op::apply(a.z, b.z), a.w = Op::apply(a.w, b.w);
+      }
+      v[4 * i] = a.x, v[4 * i + 1] = a.y, v[4 * i + 2] = a.z, v[4 * i + 3] = a.w;
+    }
+  }
+  template <int R>
+  __device__ __forceinline__ static void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[R]) {
+    if constexpr (R == 16) tmem_ld_32x16(taddr, r);
+    else
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                   : "r"(taddr));
+    tmem_ld_wait();
+  }
+  template <int R>
+  __device__ __forceinline__ static void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[R]) {
+    if constexpr (R == 16) tmem_st_32x16(taddr, r);
+    else
+      asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                   "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                   : "memory");
+    tmem_st_wait();
+  }
+
+  template <int R>   // rows worked on: 8 or 16
+  __device__ __forceinline__ static void few_tile(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice,
+                                                  int b0, int n, uint32_t tmem) {
+    const int warp = c.tid >> 5, lane = c.tid & 31, quad = (threadIdx.x >> 5) & 3, at = quad * 32 + lane;   // key of the block, then dim
+    const bool mine = warp < 4;
+    const int rows = t.npos * p.group;
+    const uint32_t tlane = tmem + ((uint32_t)(quad * 32) << 16);
+    float m[R], l[R];   // of every row: the maximum (in powers of two) the exponentials are taken against, the same in all lanes; this key's part of the sum
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < R; ++i) m[i] = -INFINITY, l[i] = 0.f;
+    if (mine && n > 0) {
+      const float sc = p.scale_log2;
+      const int last = p.causal ? min(t.last0, t.kv_len - 1) : t.kv_len - 1;   // of the first position: every row sees up to here
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        const int key0 = (b0 + j) * kAttnKeys, key = key0 + at;
+        if (ok) ok = warp_wait(w.s_bar + 8 * (j & 1), (j >> 1) & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);   // (these four warps meet in every block: they go on together after a wait that gave up)
+        tc_fence_after();
+        uint32_t r[R];
+        tmem_ld_rows<R>(tlane + (uint32_t)(j & 1) * kAttnFewRows, r);
+        float s[R];
+        bool grown = false;
+#pragma unroll
+        for (int i = 0; i < R; ++i) s[i] = i < rows ? __uint_as_float(r[i]) * sc : -INFINITY;
+        if (key0 + kAttnKeys - 1 > last) {   // not every row sees the whole block
+          int limit = last, left = p.group;
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            if (key > limit) s[i] = -INFINITY;
+            if (--left == 0) left = p.group, limit = p.causal ? min(limit + 1, t.kv_len - 1) : limit;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) grown |= s[i] > m[i] + 8.f;
+        if (quads_any(c, grown)) {   // some row's maximum grew by more than 2^8 (or is the first): as in tile()
+          float mx[R];
+#pragma unroll
+          for (int i = 0; i < R; ++i) mx[i] = fmaxf(m[i], s[i]);
+          quads_reduce<OpMax, R>(c, w, quad, lane, mx);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float f = mx[i] == -INFINITY ? 1.f : ex2(m[i] - mx[i]);
+            m[i] = mx[i];
+            l[i] *= f;
+            mx[i] = f;
+          }
+          if (j > 0) {   // block j - 1 has to be in O
+            if (ok) ok = warp_wait(w.pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+            tc_fence_after();
+            uint32_t o[R];
+            tmem_ld_rows<R>(tlane + 128, o);
+#pragma unroll
+            for (int i = 0; i < R; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mx[i]);
+            tmem_st_rows<R>(tlane + 128, o);
+          }
+        }
+        // (S of this block stands for block j - 2's products, which read this buffer: it was issued after them)
+        const uint32_t pt = pt_smem(w, j) + (uint32_t)(at >> 6) * 2048u + (uint32_t)(at & 7) * 2u;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float e = ex2(s[i] - (m[i] == -INFINITY ? 0.f : m[i]));
+          l[i] += e;
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(pt + (uint32_t)(i * 128 + ((((at & 63) >> 3) ^ (i & 7)) << 4))), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(e)))
+                       : "memory");
+        }
+        const int have = t.kv_len - key0;
+        if (have < kAttnKeys) {
+          // (these threads may be a block ahead: V's barrier says which block it holds only once block j - 1 is through)
+          if (j > 0 && ok) ok = warp_wait(w.pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          if (ok) ok = clear_tail(p, c, w, j, have, at, 128);
+        }
+        fence_async_smem();
+        tc_fence_before();
+        mbar_arrive(w.p_bar + 8 * (j & 1));
+      }
+      if (ok) ok = warp_wait(w.o_bar, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+      tc_fence_after();
+      quads_reduce<OpSum, R>(c, w, quad, lane, l);
+    }
+    uint32_t o[R];
+    auto read_o = [&] {
+#pragma unroll
+      for (int i = 0; i < R; ++i) o[i] = 0u;
+      if (n > 0) tmem_ld_rows<R>(tlane + 128, o);
+    };
+    if (split == 1) {
+      if (!mine || !ok) return;
+      read_o();
+      if (at < p.dim)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (i < rows) reinterpret_cast<__nv_bfloat16 *>(out_row(p, t, head, i))[at] = __float2bfloat16_rn(l[i] == 0.f ? 0.f : __uint_as_float(o[i]) / l[i]);
+      return;
+    }
+    // the slices become one: rank r owns the dims [r * per, (r + 1) * per)
+    cluster_sync_all();
+    if (!mine) return;
+    const int dims = w.chunks * 64, per = dims / split;
+    const uint32_t area = w.q, recv = area + 1024u;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (at == i)
+        for (int r = 0; r < split; ++r) st_async_f2(peer_smem(area + (uint32_t)(slice * kAttnFewRows + i) * 8, r), peer_smem(w.stats_bar, r), m[i], l[i]);
+    if (!warp_wait(w.stats_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT)) ok = false;
+    read_o();
+    if (at < dims) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float top = -INFINITY, sum = 0.f;
+        for (int r = 0; r < split; ++r) top = fmaxf(top, ld_shared_f2(area + (uint32_t)(r * kAttnFewRows + i) * 8).x);
+        if (top == -INFINITY) top = 0.f;
+        for (int r = 0; r < split; ++r) {
+          const float2 st = ld_shared_f2(area + (uint32_t)(r * kAttnFewRows + i) * 8);
+          sum += st.y * ex2(st.x - top);
+        }
+        o[i] = l[i] == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * (ex2(m[i] - top) / sum));
+      }
+      const int owner = at / per;
+      const uint32_t dst = peer_smem(recv + (uint32_t)(slice * per + at - owner * per) * 64, owner), bar = peer_smem(w.join_bar, owner);
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i) st_async_u4(dst + 16 * i, bar, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    }
+    __syncwarp();
+    if (!warp_wait(w.join_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT) || !ok) return;
+    for (int i = at; i < per * rows; i += 128) {
+      const int row = i / per, d = i - row * per;
+      float v = 0.f;
+      for (int r = 0; r < split; ++r) v += lds_f32(recv + (uint32_t)((r * per + d) * 64 + row * 4));   // rank order: the sum is deterministic
+      if (slice * per + d < p.dim) reinterpret_cast<__nv_bfloat16 *>(out_row(p, t, head, row))[slice * per + d] = __float2bfloat16_rn(v);
+    }
+  }
 };
+
+using AttentionBf16 = Attention<1>;
+using AttentionBf16Two = Attention<2>;
 
 }  // namespace bfuse

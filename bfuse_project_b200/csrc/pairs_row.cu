@@ -75,16 +75,17 @@ void fill_pair_row<BFUSE_ROW>(PairEntry *row, SingleEntry *single) {
   if constexpr (std::is_same<A, ConvAnyTf32>::value) {
     single->launch = &launch_single<ConvUmmaTf32>;
     single->attr = &attr_single<ConvUmmaTf32>;
-    single->launch_planes = &launch_single<A>;
+    single->launch_other = &launch_single<A>;
   } else {
     single->launch = &launch_single<A>;
     single->attr = &attr_single<A>;
-    single->launch_planes = nullptr;
+    single->launch_other = nullptr;
+    if constexpr (std::is_same<A, AttentionBf16>::value) single->launch_other = &launch_single<AttentionBf16Two>;
   }
   single->group = &launch_group<A>;
   single->group_attr = &attr_group<A>;
   single->group_clusters = &clusters_group<A>;
-  single->max_threads = A::kMaxThreads;
+  single->max_threads = std::is_same<A, AttentionBf16>::value ? AttentionBf16Two::kMaxThreads : A::kMaxThreads;
   single->params_size = sizeof(typename A::Params);
 }
 

@@ -238,23 +238,32 @@ const char *attention_problem(const bfuse_kernel_desc &d) {
   if (s[6] < 0 || s[7] < 0 || s[6] % 8 || s[7] % 8) return "strides must be multiples of 8 elements";
   if ((s[6] && s[6] < (long long)s[3] * s[5]) || (s[7] && s[7] < (long long)s[4] * s[5])) return "a stride is shorter than a token's heads";
   if (s[8] != 0 && s[8] != 1 && s[8] != 2 && s[8] != 4 && s[8] != 8) return "shape[8] (key slices) must be 1, 2, 4 or 8";
+  if (s[9] < 0 || s[9] > 2 || (s[9] == 2 && s[8] > 1)) return "shape[9] (tiles per CTA) must be 1, or 2 with one key slice";
   if (!(d.fparam[0] > 0.f) || !(d.fparam[0] < 1e30f)) return "the scale must be positive and finite";
   const int positions = kAttnRows / (s[3] / s[4]);
   const long long tiles = ((long long)s[1] + (long long)s[0] * (positions - 1)) / positions;
   if (tiles * s[4] * 8 > 0x7fffffffLL) return "more tiles than a grid holds";
   return nullptr;
 }
-// tiles at most: sum of ceil(len / P) over the sequences
-long long attention_tiles(const int *s) {
-  const int positions = kAttnRows / (s[3] / s[4]);
+// tiles (of `two` tiles: pairs) at most: sum of ceil(len / P) over the sequences
+long long attention_tiles(const int *s, int two) {
+  const int positions = kAttnRows / (s[3] / s[4]) * two;
   return ((long long)s[1] + (long long)s[0] * (positions - 1)) / positions;
 }
+// Two tiles per CTA, which load K and V once for both: alone in its launch, once there are more tiles than SMs and the
+// average sequence fills more than one.  (Two one-tile CTAs an SM pull 9 TB/s out of L2 and are bound by it.)
+bool attention_two(const int *s, int share, int sm) {
+  if (s[9] > 0) return s[9] == 2;
+  const int positions = kAttnRows / (s[3] / s[4]);
+  return share == 1 && s[8] <= 1 && attention_tiles(s, 1) * s[4] > sm && (long long)s[1] > (long long)s[0] * positions;
+}
+constexpr size_t kAttnHalfSm = 113 * 1024;   // above this window one CTA fits an SM
 int attention_min_stages(int dim, int split) { return std::max(2, ceil_div(attn_join_bytes(dim, split), attn_tile_bytes(dim)) - 1); }
 // Slices of a tile's keys: while the tiles alone leave SMs idle and every slice keeps two blocks of the average sequence.
 // Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
 int attention_slices(const int *s, int share, int sm) {
   if (s[8] > 0) return s[8];
-  const long long base = attention_tiles(s) * s[4] * share, blocks = ceil_div(s[2], s[0] * kAttnKeys);
+  const long long base = attention_tiles(s, 1) * s[4] * share, blocks = ceil_div(s[2], s[0] * kAttnKeys);
   for (int split = share == 1 ? 8 : 4; split > 1; split = share == 1 ? split / 2 : 1)
     if (base * split <= 2 * sm && blocks >= 2 * split) return split;
   return 1;
@@ -296,12 +305,12 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
     }
     case BFUSE_OP_ATTENTION_BF16: {
       if (const char *m = attention_problem(*d)) { *err = std::string("attention: ") + m; return BFUSE_ERR_SHAPE; }
-      const long long tiles = attention_tiles(s);
-      const int split = attention_slices(s, share, sm);
-      d->shape[8] = split;
-      const int budget = (long long)share * tiles * s[4] * split <= sm ? 200 * 1024 : 110 * 1024;
-      const int stages = std::max(attention_min_stages(s[5], split), std::min(kAttnMaxStages, (budget - kUmmaHeaderBytes) / attn_tile_bytes(s[5]) - 1));
-      set(split * s[4], (int)tiles, 1, kAttnThreads, 1, attn_smem_bytes(s[5], stages), 6);
+      const int two = attention_two(s, share, sm) ? 2 : 1, split = two == 2 ? 1 : attention_slices(s, share, sm);
+      const long long tiles = attention_tiles(s, two);
+      d->shape[8] = split, d->shape[9] = two;
+      const int budget = two == 2 || share * tiles * s[4] * split <= sm ? 200 * 1024 : 110 * 1024;
+      const int stages = std::max(attention_min_stages(s[5], split), std::min(kAttnMaxStages, (budget - kUmmaHeaderBytes) / attn_tile_bytes(s[5]) - two));
+      set(split * s[4], (int)tiles, 1, attn_threads(two), 1, attn_smem_bytes(s[5], two, stages), 6);
       return BFUSE_OK;
     }
     case BFUSE_OP_ROPE_BF16: {
@@ -738,11 +747,11 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
     }
     case BFUSE_OP_ATTENTION_BF16: {
       if (const char *m = attention_problem(d)) return shape_err(m);
-      const int split = s[8] > 0 ? s[8] : 1, group = s[3] / s[4], positions = kAttnRows / group;
-      if (kd.bx != kAttnThreads || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1)");
-      if (kd.gx != split * s[4] || kd.gy != attention_tiles(s) || kd.gz != 1)
-        return shape_err("GridDim must be (key slices * kv heads, (total_q + seqs * (P - 1)) / P, 1) with P = 128 / (heads / kv heads) positions a tile");
-      if (k.smem < (size_t)attn_smem_bytes(s[5], attention_min_stages(s[5], split)))
+      const int split = s[8] > 0 ? s[8] : 1, two = s[9] > 0 ? s[9] : 1, group = s[3] / s[4], positions = kAttnRows / group;
+      if (kd.bx != attn_threads(two) || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1), or (320, 1, 1) with two tiles per CTA");
+      if (kd.gx != split * s[4] || kd.gy != attention_tiles(s, two) || kd.gz != 1)
+        return shape_err("GridDim must be (key slices * kv heads, (total_q + seqs * (P - 1)) / P, 1) with P = 128 / (heads / kv heads) positions a tile, twice that with two tiles per CTA");
+      if (k.smem < (size_t)attn_smem_bytes(s[5], two, attention_min_stages(s[5], split)))
         return shape_err("shared memory below the queries and two blocks of keys or values (and, with key slices, what they exchange)");
       k.cluster = split;
       AttentionParams p;
@@ -757,7 +766,10 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       p.seqs = s[0], p.total_q = s[1], p.total_kv = s[2], p.heads = s[3], p.kv_heads = s[4], p.dim = s[5];
       p.group = group, p.positions = positions;
       p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL), p.split = split;
-      p.stages = std::min<int>(kAttnMaxStages, (int)((k.smem - kUmmaHeaderBytes) / attn_tile_bytes(s[5])) - 1);
+      p.stages = std::min<int>(kAttnMaxStages, (int)((k.smem - kUmmaHeaderBytes) / attn_tile_bytes(s[5])) - two);
+      // one CTA an SM and alone in its launch: all of tensor memory
+      p.tmem_cols = two == 2 || (((d.flags >> 8) & 7u) == 1 && k.smem > kAttnHalfSm) ? 512 : 256;
+      p.p_col = s[5] <= 64 ? 192 : p.tmem_cols == 512 && two == 1 ? 256 : 0;
       p.scale_log2 = d.fparam[0] * 1.4426950408889634f;
       static_assert(sizeof(p) <= kParamsBytes, "parameter block too small");
       std::memcpy(k.params, &p, sizeof(p));
@@ -917,6 +929,10 @@ bool takes_runs(const FusionRec &f) { return f.launch.per_cta[0] > 1 || f.launch
 // Is the kernel a conv staged as whole planes?
 bool whole_planes(const KernelRec &k) { return k.desc.op == BFUSE_OP_CONV2D_TF32 && reinterpret_cast<const ConvUmmaParams *>(k.params)->plane_imgs > 0; }
 
+// Is the kernel attention in a form that has an SM to itself (two tiles per CTA, or all of tensor memory)?  Shared launches take
+// it with one tile per CTA, 256 columns and one key slice.
+bool lone_attention(const KernelRec &k) { return k.desc.op == BFUSE_OP_ATTENTION_BF16 && reinterpret_cast<const AttentionParams *>(k.params)->tmem_cols > 256; }
+
 DispatchTable single_table(const bfuse_context *ctx, const KernelRec &k) {
   DispatchTable t;
   std::memset(&t, 0, sizeof(t));
@@ -936,7 +952,7 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
   const DispatchTable t = single_table(ctx, k);
   const size_t smem = k.smem + 1024;
   const SingleEntry &se = ctx->singles[k.desc.op];
-  cudaError_t e = (whole_planes(k) ? se.launch_planes : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
+  cudaError_t e = (whole_planes(k) || (k.desc.op == BFUSE_OP_ATTENTION_BF16 && k.desc.shape[9] == 2) ? se.launch_other : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
   if (e != cudaSuccess) return fail_cuda(ctx, e, ("launch " + k.name).c_str());
   return BFUSE_OK;
 }
@@ -946,7 +962,7 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
 bool ring_info(const KernelRec &k, int *header, int *stage_bytes, int *min_stages, int *stages) {
   const int *s = k.desc.shape;
   if (k.desc.op == BFUSE_OP_ATTENTION_BF16) {
-    *header = kUmmaHeaderBytes + attn_tile_bytes(s[5]), *stage_bytes = attn_tile_bytes(s[5]);
+    *header = kUmmaHeaderBytes + std::max(1, s[9]) * attn_tile_bytes(s[5]), *stage_bytes = attn_tile_bytes(s[5]);
     *min_stages = attention_min_stages(s[5], std::max(1, s[8]));
     *stages = reinterpret_cast<const AttentionParams *>(k.params)->stages;
     return true;
@@ -1003,6 +1019,7 @@ int add_unsplit(bfuse_context *ctx, int reg, bool gathered, int *slot) {
   const bool conv = orig.desc.op == BFUSE_OP_CONV2D_TF32;
   const bool attention = orig.desc.op == BFUSE_OP_ATTENTION_BF16;
   alt->desc.shape[conv ? 10 : attention ? 8 : 5] = 1;
+  if (attention) alt->desc.shape[9] = 1, alt->desc.flags &= ~(7u << 8);   // tiled to share an SM
   if (!conv && !attention) alt->desc.shape[6] = 0;   // tile height: the runtime's choice for the unsplit form
   if (gathered) alt->desc.shape[9] = 0, alt->desc.shape[11] = 2;
   alt->desc.KernelName = nullptr;
@@ -1265,6 +1282,9 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
     for (int i = 0; i < 2; ++i)
       if ((*side[i])->cluster > 1)
         if (const int rc = retile(i, false)) return rc;
+  for (int i = 0; i < 2; ++i)
+    if (lone_attention(**side[i]))
+      if (const int rc = retile(i, false)) return rc;
   // Thread split lays the two windows side by side; whole planes, whose window cannot go below four weight stages and
   // two raw slots (up to 98 KB), give way to the gathered form where the sum does not fit with the rings at their shallowest.
   if (pattern == PATTERN_THREAD_SPLIT) {
@@ -1302,7 +1322,7 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
   // tensor-memory columns an operator's CTA allocates
   auto tmem_cols = [](const KernelRec &k) {
     if (is_gemm_umma(k.desc.op)) return k.desc.shape[4] * std::max(1, k.desc.shape[6] / kUmmaBM);
-    if (k.desc.op == BFUSE_OP_ATTENTION_BF16) return kAttnTmemCols;
+    if (k.desc.op == BFUSE_OP_ATTENTION_BF16) return reinterpret_cast<const AttentionParams *>(k.params)->tmem_cols;
     if (k.desc.op == BFUSE_OP_CONV2D_TF32 && (k.desc.shape[11] & 1)) return kConvTmemCols;   // staged: accumulator and operand stages
     return k.desc.op == BFUSE_OP_CONV2D_TF32 ? (k.desc.shape[9] > 0 ? k.desc.shape[9] : kConvBN) : 0;
   };
@@ -1458,7 +1478,7 @@ int bfuse_register_group(bfuse_context *ctx, const int *kernels, int n, int patt
   for (int i = 0; i < n; ++i)
     if (ks[i]->cluster > 1) narrow = narrow ? std::min(narrow, ks[i]->cluster) : ks[i]->cluster, wide = std::max(wide, ks[i]->cluster);
   for (int i = 0; i < n; ++i) {
-    if (narrow != wide && slices_optional(ctx, *ks[i])) {
+    if (lone_attention(*ks[i]) || (narrow != wide && slices_optional(ctx, *ks[i]))) {
       if (const int rc = add_unsplit(ctx, kernels[i], false, &undo.h[i])) return rc;
       g->ks[i] = undo.h[i];
       ks[i] = ctx->kernels[undo.h[i]].get();

@@ -117,6 +117,12 @@ def test_many_sequences(rt):
     run(rt, [1] * 700, [int(x) for x in rng.integers(0, 40, 700)], 4, 1, 64, True)
 
 
+def test_single_tokens_with_more_tiles_than_fit_at_once(rt):
+    # loads late and in any order: the products of a block may wait for V longer than the next block's exponentials take
+    run(rt, [1] * 48, [2048 + 37 * i for i in range(48)], 32, 8, 128, True)
+    run(rt, [2] * 40, [1500] * 40, 32, 4, 64, True)      # 16 rows a tile
+
+
 def test_large_scores_and_growing_maximum(rt):
     import torch
     # keys whose scores rise along the sequence: the running maximum moves at every block
