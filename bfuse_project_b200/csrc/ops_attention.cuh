@@ -59,8 +59,13 @@ enum AttnStatus : int {
 
 __host__ __device__ constexpr int attn_chunks(int dim) { return dim <= 64 ? 1 : 2; }   // 64-element chunks of a head
 __host__ __device__ constexpr int attn_tile_bytes(int dim) { return attn_chunks(dim) * kAttnChunkBytes; }
-__host__ __device__ constexpr int attn_smem_bytes(int dim, int tiles, int stages) { return kUmmaHeaderBytes + (tiles + stages) * attn_tile_bytes(dim); }
-// what the slices of a tile exchange at the end: (m, l) per rank and row, and per 16 owned columns 8 KB of every rank
+// behind the ring, with key slices: what the ranks push to one another for a tile of few rows, (m, l) of 16 rows from each of 8
+// and 128 dims of 16 rows
+__host__ __device__ constexpr int attn_few_join_bytes(int split) { return split > 1 ? 8 * 16 * 8 + 128 * 16 * 4 : 0; }
+__host__ __device__ constexpr int attn_smem_bytes(int dim, int tiles, int stages, int split) {
+  return kUmmaHeaderBytes + (tiles + stages) * attn_tile_bytes(dim) + attn_few_join_bytes(split);
+}
+// what the slices of a whole tile exchange at the end, over Q and the ring: (m, l) per rank and row, and per 16 owned columns 8 KB of every rank
 __host__ __device__ constexpr int attn_join_bytes(int dim, int split) {
   return split > 1 ? split * kAttnRows * 8 + ((attn_chunks(dim) * 4 + split - 1) / split) * split * 16 * kAttnRows * 4 : 0;
 }
@@ -74,6 +79,7 @@ struct AttentionParams {
   int seqs, total_q, total_kv, heads, kv_heads, dim;
   int group, positions;            // query heads per kv head; positions of a tile
   int causal, split, stages;
+  int sort;                        // longest sequences first
   int tmem_cols, p_col;            // tensor memory: columns in all; first column of p, 0: over the scores
   float scale_log2;                // scale * log2(e), positive
 };
@@ -145,31 +151,69 @@ struct Attention {
   struct Window {
     // s_bar, pv_bar, o_bar, c_bar: one per tile, p_bar: two per tile (few rows: two s_bar and p_bar, by the parity of the block)
     uint32_t full0, empty0, q_bar, s_bar, p_bar, pv_bar, o_bar, c_bar, stats_bar, join_bar;
-    uint32_t xch, q, ring;
+    uint32_t xch, q, ring, few_join;
     int chunks, tile_bytes;
   };
   static constexpr int kBars = 2 * kAttnMaxStages + 15;
 
-  // Tile number t of the batch (T = 2: pair of tiles): sequence i has ceil(len_i / (T P)) of them.  One warp; 256 sequences a round, 8 a lane,
-  // so that a batch of single tokens costs one trip to memory for its offsets and not one per 32 sequences.
-  __device__ __forceinline__ static AttnTile find_tile(const Params &p, int t, int lane, int *status) {
+  // Tile number t of the batch (T = 2: pair of tiles) into *tile: sequence i has ceil(len_i / (T P)) of them, the last
+  // positions first.  One warp.  Up to 32 sequences: one a lane, the longest first where `sort` (more tiles than run at
+  // once: a long sequence that starts late ends last); more: 256 a round, 8 a lane.
+  __device__ __forceinline__ static void find_tile(const Params &p, int t, int lane, AttnTile *tile, int *status) {
     const int positions = T * p.positions;
-    AttnTile tile;
-    tile.found = 0;
+    auto bad = [&] { atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS); };
+    auto put = [&](int q0, int q_len, int kv0, int kv_end, int qt) {
+      AttnTile r;
+      r.found = kv0 >= 0 && kv_end >= kv0 && kv_end <= p.total_kv;
+      if (!r.found) bad();
+      r.q0 = q0 + qt * positions;
+      r.npos = min(positions, q_len - qt * positions);
+      r.kv0 = kv0;
+      r.kv_len = kv_end - kv0;
+      r.last0 = r.kv_len - q_len + qt * positions;
+      r.keys = p.causal ? max(0, min(r.kv_len, r.last0 + r.npos)) : r.kv_len;
+      *tile = r;
+    };
+    if (lane == 0) tile->found = 0;
+    __syncwarp();
+    if (p.seqs <= 32) {
+      const int s0 = min(lane, p.seqs);
+      const int qa = __ldg(p.cu_q + s0), ka = __ldg(p.cu_kv + s0), qb = __ldg(p.cu_q + min(s0 + 1, p.seqs)), kb = __ldg(p.cu_kv + min(s0 + 1, p.seqs));
+      int n = 0;
+      if (lane < p.seqs) {
+        if (qa < 0 || qb < qa || qb > p.total_q) bad();
+        else n = (qb - qa + positions - 1) / positions;
+      }
+      int at = 0;   // first tile of this lane's sequence
+      if (p.sort) {
+        for (int i = 0; i < p.seqs; ++i) {
+          const int m = __shfl_sync(0xffffffffu, n, i);
+          if (m > n || (m == n && i < lane)) at += m;
+        }
+      } else {
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, off);
+          if (lane >= off) upto += v;
+        }
+        at = upto - n;
+      }
+      if (t >= at && t < at + n) put(qa, qb - qa, ka, kb, n - 1 - (t - at));
+      __syncwarp();
+      return;
+    }
     int before = 0;   // tiles of the sequences before this round's
     for (int base = 0; base < p.seqs; base += 256) {
       const int s0 = base + lane * 8;
-      int cu[9], kv[9], n[8], mine = 0;
+      int cu[9], n[8], mine = 0;
 #pragma unroll
-      for (int i = 0; i < 9; ++i) {
-        cu[i] = s0 + i <= p.seqs ? __ldg(p.cu_q + s0 + i) : 0;
-        kv[i] = s0 + i <= p.seqs ? __ldg(p.cu_kv + s0 + i) : 0;
-      }
+      for (int i = 0; i < 9; ++i) cu[i] = __ldg(p.cu_q + min(s0 + i, p.seqs));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         n[i] = 0;
         if (s0 + i < p.seqs) {
-          if (cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > p.total_q) atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS);
+          if (cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] > p.total_q) bad();
           else n[i] = (cu[i + 1] - cu[i] + positions - 1) / positions;
         }
         mine += n[i];
@@ -183,45 +227,27 @@ struct Attention {
       const int total = __shfl_sync(0xffffffffu, upto, 31);
       if (t - before < total) {
         int at = before + upto - mine;   // first tile of this lane's sequences
-        const bool here = t >= at && t < at + mine;
-        if (here) {
-          bool done = false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (!done && t < at + n[i]) {
-              done = true;
-              const int qt = n[i] - 1 - (t - at);   // the last positions first
-              const int q_len = cu[i + 1] - cu[i];
-              tile.found = kv[i] >= 0 && kv[i + 1] >= kv[i] && kv[i + 1] <= p.total_kv;
-              if (!tile.found) atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS);
-              tile.q0 = cu[i] + qt * positions;
-              tile.npos = min(positions, q_len - qt * positions);
-              tile.kv0 = kv[i];
-              tile.kv_len = kv[i + 1] - kv[i];
-              tile.last0 = tile.kv_len - q_len + qt * positions;
-              tile.keys = p.causal ? max(0, min(tile.kv_len, tile.last0 + tile.npos)) : tile.kv_len;
-            }
-            at += n[i];
-          }
+        for (int i = 0; i < 8; ++i) {
+          if (t >= at && t < at + n[i]) put(cu[i], cu[i + 1] - cu[i], __ldg(p.cu_kv + s0 + i), __ldg(p.cu_kv + s0 + i + 1), n[i] - 1 - (t - at));
+          at += n[i];
         }
-        const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-        tile.found = __shfl_sync(0xffffffffu, tile.found, src);
-        tile.q0 = __shfl_sync(0xffffffffu, tile.q0, src);
-        tile.npos = __shfl_sync(0xffffffffu, tile.npos, src);
-        tile.kv0 = __shfl_sync(0xffffffffu, tile.kv0, src);
-        tile.kv_len = __shfl_sync(0xffffffffu, tile.kv_len, src);
-        tile.last0 = __shfl_sync(0xffffffffu, tile.last0, src);
-        tile.keys = __shfl_sync(0xffffffffu, tile.keys, src);
-        return tile;
+        __syncwarp();
+        return;
       }
       before += total;
     }
-    return tile;
+  }
+
+  // of the barriers from q_bar on, those that the 128 threads of a tile arrive at: p_bar (four) and c_bar (two)
+  __device__ __forceinline__ static bool by_threads(const Window &w, int i) {
+    const uint32_t bar = w.q_bar + 8 * i;
+    return (bar >= w.p_bar && bar < w.pv_bar) || (bar >= w.c_bar && bar < w.stats_bar);
   }
 
   // this slice's blocks of keys: first and count
   __device__ __forceinline__ static void my_blocks(const AttnTile &t, int split, int slice, int &b0, int &n) {
-    const int nblocks = (t.keys + kAttnKeys - 1) / kAttnKeys, per = (nblocks + split - 1) / split;
+    const int nblocks = (t.keys + kAttnKeys - 1) / kAttnKeys, per = (nblocks + split - 1) >> log2_of(split);   // (a power of two)
     b0 = min(nblocks, slice * per);
     n = min(nblocks, b0 + per) - b0;
   }
@@ -264,12 +290,12 @@ struct Attention {
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
     const int warp = c.tid >> 5, lane = c.tid & 31;
     const int split = p.split, stages = p.stages;
-    const int bx = c.block_x(), slice = bx % split, head = bx / split;
+    const int bx = c.block_x(), slice = bx & (split - 1), head = bx >> log2_of(split);   // (split: a power of two)
     Window w;
     w.full0 = smem_u32(c.smem), w.empty0 = w.full0 + 8 * kAttnMaxStages, w.q_bar = w.empty0 + 8 * kAttnMaxStages;
     w.s_bar = w.q_bar + 8, w.p_bar = w.q_bar + 24, w.pv_bar = w.q_bar + 56, w.o_bar = w.q_bar + 72, w.c_bar = w.q_bar + 88, w.stats_bar = w.q_bar + 104, w.join_bar = w.q_bar + 112;
     w.xch = w.full0 + 1024, w.q = w.full0 + kUmmaHeaderBytes;
-    w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes;
+    w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes, w.few_join = w.ring + stages * w.tile_bytes;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * kBars);
     AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 256);
 
@@ -279,46 +305,28 @@ struct Attention {
     }
     int loaded = 0;
     if (warp == kProducer) {
+      // all of this needs no memory: it runs while the previous kernel ends
       if (lane < stages) {
         mbar_init(w.full0 + 8 * lane, 1);
         mbar_init(w.empty0 + 8 * lane, 1);
       }
-      if (lane == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_q) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_k) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.map_v) : "memory");
-      }
+      if (lane < kBars - 2 * kAttnMaxStages) mbar_init(w.q_bar + 8 * lane, by_threads(w, lane) ? 128 : 1);
+      if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_q : lane == 1 ? &p.map_k : &p.map_v) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       c.dependency_wait();
-      const AttnTile t = find_tile(p, c.block_y(), lane, c.status);
+      find_tile(p, c.block_y(), lane, tile_slot, c.status);
+      const AttnTile t = *tile_slot;
       const bool few = t.found && few_rows(p, t);
       const int active = t.found ? (sub_tile(p, t, 0).npos * p.group + 31) >> 5 : 0;   // quarters of the (first) tile that hold a row
       int b0 = 0, n = 0;
       if (t.found) my_blocks(t, split, slice, b0, n);
-      if (lane == 0) {
-        *tile_slot = t;
-        mbar_init(w.q_bar, 1);
-        mbar_init(w.stats_bar, 1);
-        mbar_init(w.join_bar, 1);
-        for (int x = 0; x < 2; ++x) {
-          const int threads = few ? 128 : x == 0 || T == 1 ? active * 32 : t.found ? (sub_tile(p, t, x).npos * p.group + 31) & ~31 : 0;
-          mbar_init(w.s_bar + 8 * x, 1);
-          mbar_init(w.pv_bar + 8 * x, 1);
-          mbar_init(w.o_bar + 8 * x, 1);
-          mbar_init(w.c_bar + 8 * x, max(threads, 1));
-          mbar_init(w.p_bar + (T == 1 ? 8 : 16) * x, max(threads, 1));
-          if (T == 2) mbar_init(w.p_bar + 16 * x + 8, max(threads, 1));
-        }
-      }
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      __syncwarp();
       loaded = min(stages, 2 * n);
       if (elect_one()) {
         if (split > 1 && t.found) {
           // what this CTA will receive: (m, l) of every row from every rank, and the columns (few rows: dims) that it owns
           if (few) {
             const int r = t.npos * p.group <= 8 ? 8 : kAttnFewRows;
-            mbar_expect_tx(w.stats_bar, (uint32_t)(split * r * 8));
-            mbar_expect_tx(w.join_bar, (uint32_t)(w.chunks * 64 * r * 4));
+            mbar_expect_tx(w.join_bar, (uint32_t)(split * r * 8 + w.chunks * 64 * r * 4));
           } else {
             int owned = 0;
             for (int ch = slice; ch < w.chunks * 4; ch += split) ++owned;
@@ -342,6 +350,8 @@ struct Attention {
     tc_fence_before();
     c.sync();
     tc_fence_after();
+    // this CTA's barriers are up: its peers may push (they wait for that only when they have something to push)
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const uint32_t tmem = c.tmem_given ? c.tmem_base : *reinterpret_cast<volatile uint32_t *>(tmem_slot);
     const AttnTile t = *tile_slot;
     if (t.found) {   // (the same for every CTA of a cluster)
@@ -386,6 +396,8 @@ struct Attention {
       } else {
         tile(p, c, w, t, head, split, slice, b0, n, tmem, 0);
       }
+    } else if (split > 1) {
+      cluster_wait();
     }
     __syncwarp();
     tc_fence_before();
@@ -401,6 +413,8 @@ struct Attention {
   // groups of 8 keys 1024 bytes (stride offset), 16 keys -- one instruction -- 2048
   __device__ __forceinline__ static uint32_t v_desc(uint32_t addr, uint32_t chunk_step) { return ((addr >> 4) & 0x3fffu) | ((chunk_step >> 4) << 16); }
   __device__ __forceinline__ static uint32_t k_major_desc(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+
+  __device__ __forceinline__ static void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
   // ---- whole tiles: rows in the lanes ----
 
@@ -559,10 +573,19 @@ struct Attention {
     const int warp = c.tid >> 5, lane = c.tid & 31;
     const int quad = (threadIdx.x >> 5) & 3;   // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
     const int rows = t.npos * p.group, row = quad * 32 + lane, active = (rows + 31) >> 5;
-    const bool mine = warp < kProducer && quad < active;   // this warp owns rows
+    const bool mine = warp < kProducer && quad < active;   // this warp owns rows (the others only keep the barriers going)
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
     float m = -INFINITY, l = 0.f;   // the maximum the exponentials are taken against, and their sum
     bool ok = true;
+    if (!mine && warp < kProducer) {
+      for (int j = 0; j < n && ok; ++j) {
+        ok = warp_wait(w.s_bar + 8 * x, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        if (p.p_col) mbar_arrive(w.c_bar + 8 * x);
+        if (p.p_col && j > 0 && ok) ok = warp_wait(w.pv_bar + 8 * x, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+        mbar_arrive(w.p_bar + 16 * x);
+        mbar_arrive(w.p_bar + 16 * x + 8);
+      }
+    }
     if (mine && n > 0) {
       const int limit = row < rows ? (p.causal ? min(t.last0 + row / p.group, t.kv_len - 1) : t.kv_len - 1) : -1;   // last key this row sees
       const float sc = p.scale_log2;
@@ -627,8 +650,10 @@ struct Attention {
     if (T == 1 && split > 1) {
       join(p, c, w, t, head, split, slice, n, rows, row, mine, ok, trow, m, l);
     } else if (mine && ok) {
-      uint16_t *out = out_row(p, t, head, row);
+      // Through the rows of the Q tile, which no MMA reads any more (swizzled as the TMA left them), so that a row's dims leave
+      // as whole lines: thread by thread, 16 bytes of 32 rows at a time, the stores took 2600 clocks of 128 dims, so 600.
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const uint32_t stage = w.q + x * w.tile_bytes + (uint32_t)(quad * 32) * 128u;
 #pragma unroll 1
       for (int col = 0; col < p.dim; col += 32) {
         uint32_t r[32];
@@ -636,15 +661,29 @@ struct Attention {
           tmem_ld_32x32(trow + 128 + col, r);
           tmem_ld_wait();
         }
-        if (row < rows) {
-          float v[16];
+        const uint32_t line = stage + (uint32_t)(col >> 6) * kAttnChunkBytes + (uint32_t)lane * 128u;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int i = 0; i < 4; ++i) {
+          float v[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = l == 0.f ? 0.f : __uint_as_float(r[16 * h + j]) * inv;   // a row without keys: zeros
-            store16(out, col + 16 * h, p.dim, v);
-          }
+          for (int k = 0; k < 8; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(r[8 * i + k]) * inv;   // a row without keys: zeros
+          st_shared_u4(line + (uint32_t)(((((col >> 3) & 7) + i) ^ (lane & 7)) << 4), f2_to_bf16x2(v[0], v[1]), f2_to_bf16x2(v[2], v[3]),
+                       f2_to_bf16x2(v[4], v[5]), f2_to_bf16x2(v[6], v[7]));
         }
+      }
+      __syncwarp();
+      const int per_row = p.dim >> 3, lanes = per_row <= 8 ? 8 : 16, sub = lane & (lanes - 1);   // 16-byte pieces of a row; lanes that share one
+      const int i0 = lanes == 8 ? lane >> 3 : lane >> 4, step = 32 / lanes;
+      int g = quad * 32 + i0, pos = g / p.group;   // of the first row: head of the group, position
+      g -= pos * p.group;
+      uint16_t *out = p.out + ((size_t)(t.q0 + pos) * p.heads + head * p.group + g) * p.dim + 8 * sub;
+      const size_t next = (size_t)(p.heads - p.group) * p.dim;   // from the group's heads to those of the next position
+#pragma unroll 4
+      for (int i = i0; i < 32; i += step) {
+        if (sub < per_row && quad * 32 + i < rows)
+          *reinterpret_cast<float4 *>(out) = ld_shared_f4(stage + (uint32_t)(sub >> 3) * kAttnChunkBytes + (uint32_t)i * 128u + (uint32_t)(((sub & 7) ^ (i & 7)) << 4));
+        out += step * p.dim;
+        for (g += step; g >= p.group; g -= p.group) out += next;
       }
     }
   }
@@ -652,6 +691,7 @@ struct Attention {
   // The slices of a tile become one result (all threads of every CTA of the cluster).
   __device__ __forceinline__ static void join(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice, int n,
                                               int rows, int row, bool mine, bool ok, uint32_t trow, float m, float l) {
+    cluster_wait();
     cluster_sync_all();   // every rank's MMAs are done: Q and the ring are free everywhere
     if (!mine) return;
     const float mlog = m * p.scale_log2;   // in powers of two
@@ -895,40 +935,47 @@ struct Attention {
           if (i < rows) reinterpret_cast<__nv_bfloat16 *>(out_row(p, t, head, i))[at] = __float2bfloat16_rn(l[i] == 0.f ? 0.f : __uint_as_float(o[i]) / l[i]);
       return;
     }
-    // the slices become one: rank r owns the dims [r * per, (r + 1) * per)
-    cluster_sync_all();
+    // The slices become one: rank r owns the dims [r * per, (r + 1) * per).  Everyone pushes (m, l) of its rows to all and its
+    // part of O, as it is, to the owners, into memory kept for that; the owner weighs the parts.
+    cluster_wait();
     if (!mine) return;
-    const int dims = w.chunks * 64, per = dims / split;
-    const uint32_t area = w.q, recv = area + 1024u;
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (at == i)
-        for (int r = 0; r < split; ++r) st_async_f2(peer_smem(area + (uint32_t)(slice * kAttnFewRows + i) * 8, r), peer_smem(w.stats_bar, r), m[i], l[i]);
-    if (!warp_wait(w.stats_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT)) ok = false;
+    const int dims = w.chunks * 64, per_log2 = log2_of(dims) - log2_of(split), per = 1 << per_log2;
+    const uint32_t stats = w.few_join, recv = stats + 1024u;
     read_o();
     if (at < dims) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        float top = -INFINITY, sum = 0.f;
-        for (int r = 0; r < split; ++r) top = fmaxf(top, ld_shared_f2(area + (uint32_t)(r * kAttnFewRows + i) * 8).x);
-        if (top == -INFINITY) top = 0.f;
-        for (int r = 0; r < split; ++r) {
-          const float2 st = ld_shared_f2(area + (uint32_t)(r * kAttnFewRows + i) * 8);
-          sum += st.y * ex2(st.x - top);
-        }
-        o[i] = l[i] == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * (ex2(m[i] - top) / sum));
-      }
-      const int owner = at / per;
-      const uint32_t dst = peer_smem(recv + (uint32_t)(slice * per + at - owner * per) * 64, owner), bar = peer_smem(w.join_bar, owner);
+      const int owner = at >> per_log2;
+      const uint32_t dst = peer_smem(recv + (uint32_t)(slice * per + at - owner * per) * (R * 4), owner), bar = peer_smem(w.join_bar, owner);
 #pragma unroll
       for (int i = 0; i < R / 4; ++i) st_async_u4(dst + 16 * i, bar, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
     }
+#pragma unroll
+    for (int i = 0; i < R; ++i)   // lane r of quarter i % 4 tells rank r of row i
+      if (quad == (i & 3) && lane < split) st_async_f2(peer_smem(stats + (uint32_t)(slice * R + i) * 8, lane), peer_smem(w.join_bar, lane), m[i], l[i]);
     __syncwarp();
-    if (!warp_wait(w.join_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT) || !ok) return;
+    if (!warp_wait(w.join_bar, 0, c.status, ATTN_WAIT_PEERS_TIMEOUT)) ok = false;
+    if (at < R) {   // what the ranks' parts of row `at` count
+      float top = -INFINITY, sum = 0.f;
+      for (int r = 0; r < split; ++r) top = fmaxf(top, ld_shared_f2(stats + (uint32_t)(r * R + at) * 8).x);
+      if (top == -INFINITY) top = 0.f;
+      for (int r = 0; r < split; ++r) {
+        const float2 st = ld_shared_f2(stats + (uint32_t)(r * R + at) * 8);
+        sum += st.y * ex2(st.x - top);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      for (int r = 0; r < split; ++r) {
+        const float2 st = ld_shared_f2(stats + (uint32_t)(r * R + at) * 8);
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.xch + (uint32_t)(r * R + at) * 4), "f"(st.y == 0.f ? 0.f : ex2(st.x - top) * inv) : "memory");
+      }
+    }
+    quads_sync(c);
+    if (!ok) return;
     for (int i = at; i < per * rows; i += 128) {
-      const int row = i / per, d = i - row * per;
+      const int row = i >> per_log2, d = i & (per - 1);
       float v = 0.f;
-      for (int r = 0; r < split; ++r) v += lds_f32(recv + (uint32_t)((r * per + d) * 64 + row * 4));   // rank order: the sum is deterministic
+      for (int r = 0; r < split; ++r) {   // rank order: the sum is deterministic
+        const float f = lds_f32(w.xch + (uint32_t)(r * R + row) * 4);
+        if (f != 0.f) v = fmaf(f, lds_f32(recv + (uint32_t)((r * per + d) * R + row) * 4), v);
+      }
       if (slice * per + d < p.dim) reinterpret_cast<__nv_bfloat16 *>(out_row(p, t, head, row))[slice * per + d] = __float2bfloat16_rn(v);
     }
   }

@@ -251,21 +251,22 @@ long long attention_tiles(const int *s, int two) {
   return ((long long)s[1] + (long long)s[0] * (positions - 1)) / positions;
 }
 // Two tiles per CTA, which load K and V once for both: alone in its launch, once there are more tiles than SMs and the
-// average sequence fills more than one.  (Two one-tile CTAs an SM pull 9 TB/s out of L2 and are bound by it.)
+// average sequence fills more than one and has 2048 keys (shorter ones: two CTAs an SM hide one another's start and end).  (Two one-tile CTAs an SM pull 9 TB/s out of L2 and are bound by it.)
 bool attention_two(const int *s, int share, int sm) {
   if (s[9] > 0) return s[9] == 2;
   const int positions = kAttnRows / (s[3] / s[4]);
-  return share == 1 && s[8] <= 1 && attention_tiles(s, 1) * s[4] > sm && (long long)s[1] > (long long)s[0] * positions;
+  return share == 1 && s[8] <= 1 && attention_tiles(s, 1) * s[4] > sm && (long long)s[1] > (long long)s[0] * positions && (long long)s[2] >= 2048LL * s[0];
 }
 constexpr size_t kAttnHalfSm = 113 * 1024;   // above this window one CTA fits an SM
 int attention_min_stages(int dim, int split) { return std::max(2, ceil_div(attn_join_bytes(dim, split), attn_tile_bytes(dim)) - 1); }
-// Slices of a tile's keys: while the tiles alone leave SMs idle and every slice keeps two blocks of the average sequence.
-// Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
+// Slices of a tile's keys: while every slice still finds an SM and keeps two blocks of the average sequence (one token each for
+// 16 sequences of up to 4096 keys, 8 kv heads: 30 us with one slice and a CTA an SM, 37 with two slices and two CTAs an SM,
+// whose rings are half as deep).  Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
 int attention_slices(const int *s, int share, int sm) {
   if (s[8] > 0) return s[8];
   const long long base = attention_tiles(s, 1) * s[4] * share, blocks = ceil_div(s[2], s[0] * kAttnKeys);
   for (int split = share == 1 ? 8 : 4; split > 1; split = share == 1 ? split / 2 : 1)
-    if (base * split <= 2 * sm && blocks >= 2 * split) return split;
+    if (base * split <= sm && blocks >= 2 * split) return split;
   return 1;
 }
 
@@ -308,9 +309,9 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       const int two = attention_two(s, share, sm) ? 2 : 1, split = two == 2 ? 1 : attention_slices(s, share, sm);
       const long long tiles = attention_tiles(s, two);
       d->shape[8] = split, d->shape[9] = two;
-      const int budget = two == 2 || share * tiles * s[4] * split <= sm ? 200 * 1024 : 110 * 1024;
-      const int stages = std::max(attention_min_stages(s[5], split), std::min(kAttnMaxStages, (budget - kUmmaHeaderBytes) / attn_tile_bytes(s[5]) - two));
-      set(split * s[4], (int)tiles, 1, attn_threads(two), 1, attn_smem_bytes(s[5], two, stages), 6);
+      const int budget = (two == 2 || share * tiles * s[4] * split <= sm ? 220 : 110) * 1024;   // an SM, or half of one
+      const int stages = std::max(attention_min_stages(s[5], split), std::min(kAttnMaxStages, (budget - kUmmaHeaderBytes - attn_few_join_bytes(split)) / attn_tile_bytes(s[5]) - two));
+      set(split * s[4], (int)tiles, 1, attn_threads(two), 1, attn_smem_bytes(s[5], two, stages, split), 6);
       return BFUSE_OK;
     }
     case BFUSE_OP_ROPE_BF16: {
@@ -751,7 +752,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if (kd.bx != attn_threads(two) || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1), or (320, 1, 1) with two tiles per CTA");
       if (kd.gx != split * s[4] || kd.gy != attention_tiles(s, two) || kd.gz != 1)
         return shape_err("GridDim must be (key slices * kv heads, (total_q + seqs * (P - 1)) / P, 1) with P = 128 / (heads / kv heads) positions a tile, twice that with two tiles per CTA");
-      if (k.smem < (size_t)attn_smem_bytes(s[5], two, attention_min_stages(s[5], split)))
+      if (k.smem < (size_t)attn_smem_bytes(s[5], two, attention_min_stages(s[5], split), split))
         return shape_err("shared memory below the queries and two blocks of keys or values (and, with key slices, what they exchange)");
       k.cluster = split;
       AttentionParams p;
@@ -766,7 +767,9 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       p.seqs = s[0], p.total_q = s[1], p.total_kv = s[2], p.heads = s[3], p.kv_heads = s[4], p.dim = s[5];
       p.group = group, p.positions = positions;
       p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL), p.split = split;
-      p.stages = std::min<int>(kAttnMaxStages, (int)((k.smem - kUmmaHeaderBytes) / attn_tile_bytes(s[5])) - two);
+      // (two tiles a CTA, or a window for one CTA an SM: as many as SMs run at once, else twice that)
+      p.sort = s[0] > 1 && (long long)kd.gx * kd.gy > (two == 2 || k.smem > kAttnHalfSm ? 1 : 2) * ctx->sm_count;
+      p.stages = std::min<int>(kAttnMaxStages, (int)((k.smem - kUmmaHeaderBytes - attn_few_join_bytes(split)) / attn_tile_bytes(s[5])) - two);
       // one CTA an SM and alone in its launch: all of tensor memory
       p.tmem_cols = two == 2 || (((d.flags >> 8) & 7u) == 1 && k.smem > kAttnHalfSm) ? 512 : 256;
       p.p_col = s[5] <= 64 ? 192 : p.tmem_cols == 512 && two == 1 ? 256 : 0;
@@ -962,7 +965,7 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
 bool ring_info(const KernelRec &k, int *header, int *stage_bytes, int *min_stages, int *stages) {
   const int *s = k.desc.shape;
   if (k.desc.op == BFUSE_OP_ATTENTION_BF16) {
-    *header = kUmmaHeaderBytes + std::max(1, s[9]) * attn_tile_bytes(s[5]), *stage_bytes = attn_tile_bytes(s[5]);
+    *header = kUmmaHeaderBytes + std::max(1, s[9]) * attn_tile_bytes(s[5]) + attn_few_join_bytes(s[8]), *stage_bytes = attn_tile_bytes(s[5]);
     *min_stages = attention_min_stages(s[5], std::max(1, s[8]));
     *stages = reinterpret_cast<const AttentionParams *>(k.params)->stages;
     return true;
