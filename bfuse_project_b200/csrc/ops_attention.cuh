@@ -504,23 +504,6 @@ struct Attention {
     return v;
   }
 
-  // Two values at a time: the packed fp32 instructions do two lanes' worth in one issue slot.
-  __device__ __forceinline__ static float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-  }
-  __device__ __forceinline__ static float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-  }
-
   // Values past the end of the sequence are the next one's, or whatever the buffer holds: p is 0 there, but 0 * NaN is not,
   // so those rows of V become zeros.  `first` of `threads` threads; the block's V is load 2 j + 1 of the ring.
   __device__ __forceinline__ static bool clear_tail(const Params &p, const TileCtx &c, const Window &w, int j, int have, int first, int threads) {

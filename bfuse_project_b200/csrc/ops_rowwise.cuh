@@ -253,9 +253,13 @@ struct RmsNormBf16 {
 // ------------------------------------------------- norms after and before a block, gate, residual
 //   b' = N(b) * w_after (or b);   r = x + scale * gate * b';   y = N(r) * w_before
 // with N(v) = v / sqrt(mean(v^2) + eps): what lies between two blocks of a layer, in one pass over its rows.  x and b are
-// read once and stay in registers (in bf16, 8 values a register quad; r takes their place in fp32), r and y are written
-// once.  y is taken from r before its rounding to bf16.  Either norm, the gate and either output may be absent.
-// Any multiple of 8 columns: threads per row are a power of two and a thread's last vector may lie past the row.
+// read once and stay in registers (in bf16; r takes their place in fp32), r and y are written once.  y is taken from r before
+// its rounding to bf16.  Either norm, the gate and either output may be absent.
+// Any multiple of 8 columns: threads per row are a power of two, or with one row per CTA any number of warps, and a
+// thread's last vector may lie past the row.
+//
+// Bound by memory, and close to being bound by issuing instructions: 54 an element before the arithmetic was packed and a
+// row's missing parts were left out.
 struct ResidualNormBf16 {
   static constexpr int kRunRows = 1;
   struct Params {
@@ -275,84 +279,94 @@ struct ResidualNormBf16 {
   static constexpr bool kUsesTmem = false;
   static constexpr int kMaxVec = 4;      // 8 bf16 per vector: rows of up to 8192
 
+  __device__ __forceinline__ static float row_sum(float v, const TileCtx &c, bool whole, int slot) {
+    if (!whole || c.nthreads <= 32) return row_reduce<OpSum>(v, c, c.bx, slot);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    float *s = reinterpret_cast<float *>(c.smem) + slot * 32;
+    if ((c.tid & 31) == 0) s[c.tid >> 5] = v;
+    c.sync();
+    v = s[0];
+    for (int w = 1; w < c.nthreads >> 5; ++w) v += s[w];
+    return v;
+  }
+
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
-    const int tpr = c.bx, tsh = log2_of(tpr), lane = c.tid & (tpr - 1), row = c.vblock * c.by + (c.tid >> tsh);
+    const bool whole = c.by == 1;   // one row per CTA
+    const int tpr = c.bx, tsh = log2_of(tpr), lane = whole ? c.tid : c.tid & (tpr - 1), row = whole ? c.vblock : c.vblock * c.by + (c.tid >> tsh);
     const int nv = p.cols >> 3;   // vectors of a row
     c.dependency_wait();
     const bool live = row < p.rows;
-    const uint4 *br = reinterpret_cast<const uint4 *>(p.b + (size_t)row * p.cols), *xr = reinterpret_cast<const uint4 *>(p.x + (size_t)row * p.cols);
-    const uint4 *g4 = p.gate ? reinterpret_cast<const uint4 *>(p.gate + (size_t)(live ? row / p.gate_rows : 0) * p.cols) : nullptr;
-    const uint4 *wa4 = reinterpret_cast<const uint4 *>(p.w_after), *wb4 = reinterpret_cast<const uint4 *>(p.w_before);
+    const size_t at = (size_t)row * p.cols;
+    const uint4 *br = reinterpret_cast<const uint4 *>(p.b + at) + lane, *xr = reinterpret_cast<const uint4 *>(p.x + at) + lane;
+    const uint4 *g4 = p.gate ? reinterpret_cast<const uint4 *>(p.gate + (size_t)(live ? row / p.gate_rows : 0) * p.cols) + lane : nullptr;
+    const uint4 *wa4 = p.w_after ? reinterpret_cast<const uint4 *>(p.w_after) + lane : nullptr;
+    const uint4 *wb4 = p.w_before ? reinterpret_cast<const uint4 *>(p.w_before) + lane : nullptr;
+    const int mine = live ? nv - lane : 0;   // vector i of this thread exists while i * tpr < mine
     // every load of the row is issued before the first use of any of them (see SoftmaxF32)
     uint4 b[kMaxVec], x[kMaxVec];
 #pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-      const int k = i * tpr + lane;
-      b[i] = make_uint4(0, 0, 0, 0), x[i] = make_uint4(0, 0, 0, 0);
-      if (k < nv && live) b[i] = ld_stream_u4(br + k);
-    }
+    for (int i = 0; i < kMaxVec; ++i)
+      if (i * tpr < mine) b[i] = ld_stream_u4(br + i * tpr);
 #pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-      const int k = i * tpr + lane;
-      if (k < nv && live) x[i] = ld_stream_u4(xr + k);
-    }
-    for (int k = lane; k < nv && live; k += tpr) {
-      if (g4) prefetch_l1(g4 + k);
-      if (c.tid < tpr) {   // one row's worth of threads touches every line of the weight vectors
-        if (wa4) prefetch_l1(wa4 + k);
-        if (wb4) prefetch_l1(wb4 + k);
+    for (int i = 0; i < kMaxVec; ++i)
+      if (i * tpr < mine) x[i] = ld_stream_u4(xr + i * tpr);
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i)
+      if (i * tpr < mine) {
+        if (g4) prefetch_l1(g4 + i * tpr);
+        if (wa4 && c.tid < tpr) prefetch_l1(wa4 + i * tpr);   // one row's worth of threads touches every line of the weight vectors
+        if (wb4 && c.tid < tpr) prefetch_l1(wb4 + i * tpr);
       }
-    }
     float rinv = p.scale;
     if (wa4) {
-      float q = 0.f;
+      float2 q = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < kMaxVec; ++i) {
-        const uint32_t u[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = bf16x2_to_f2(u[j]);
-          q += f.x * f.x + f.y * f.y;
+      for (int i = 0; i < kMaxVec; ++i)
+        if (i * tpr < mine) {
+          const float2 f0 = bf16x2_to_f2(b[i].x), f1 = bf16x2_to_f2(b[i].y), f2 = bf16x2_to_f2(b[i].z), f3 = bf16x2_to_f2(b[i].w);
+          q = fma2(f3, f3, fma2(f2, f2, fma2(f1, f1, fma2(f0, f0, q))));
         }
-      }
-      rinv = p.scale / sqrtf(row_reduce<OpSum>(q, c, tpr, 0) / (float)p.cols + p.eps);
+      rinv = p.scale / sqrtf(row_sum(q.x + q.y, c, whole, 0) / (float)p.cols + p.eps);
     }
-    float r[kMaxVec][8];
-    float q = 0.f;
+    float2 r[kMaxVec][4];   // takes the registers of b and x
+    float2 q = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kMaxVec; ++i) {
-      const int k = i * tpr + lane;
-      const bool in = k < nv && live;
-      const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-      const uint4 wv = wa4 && in ? __ldg(wa4 + k) : one, gv = g4 && in ? __ldg(g4 + k) : one;
-      const uint32_t ub[4] = {b[i].x, b[i].y, b[i].z, b[i].w}, ux[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      const uint32_t uw[4] = {wv.x, wv.y, wv.z, wv.w}, ug[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 fb = bf16x2_to_f2(ub[j]), fx = bf16x2_to_f2(ux[j]), fw = bf16x2_to_f2(uw[j]), fg = bf16x2_to_f2(ug[j]);
-        r[i][2 * j] = fx.x + fb.x * rinv * fw.x * fg.x;
-        r[i][2 * j + 1] = fx.y + fb.y * rinv * fw.y * fg.y;
-        q += r[i][2 * j] * r[i][2 * j] + r[i][2 * j + 1] * r[i][2 * j + 1];
+      if (i * tpr < mine) {
+        const float2 rinv2 = make_float2(rinv, rinv);
+        r[i][0] = mul2(bf16x2_to_f2(b[i].x), rinv2), r[i][1] = mul2(bf16x2_to_f2(b[i].y), rinv2);
+        r[i][2] = mul2(bf16x2_to_f2(b[i].z), rinv2), r[i][3] = mul2(bf16x2_to_f2(b[i].w), rinv2);
+        if (wa4) {
+          const uint4 v = __ldg(wa4 + i * tpr);
+          r[i][0] = mul2(r[i][0], bf16x2_to_f2(v.x)), r[i][1] = mul2(r[i][1], bf16x2_to_f2(v.y));
+          r[i][2] = mul2(r[i][2], bf16x2_to_f2(v.z)), r[i][3] = mul2(r[i][3], bf16x2_to_f2(v.w));
+        }
+        if (g4) {
+          const uint4 v = __ldg(g4 + i * tpr);
+          r[i][0] = mul2(r[i][0], bf16x2_to_f2(v.x)), r[i][1] = mul2(r[i][1], bf16x2_to_f2(v.y));
+          r[i][2] = mul2(r[i][2], bf16x2_to_f2(v.z)), r[i][3] = mul2(r[i][3], bf16x2_to_f2(v.w));
+        }
+        r[i][0] = add2(r[i][0], bf16x2_to_f2(x[i].x)), r[i][1] = add2(r[i][1], bf16x2_to_f2(x[i].y));
+        r[i][2] = add2(r[i][2], bf16x2_to_f2(x[i].z)), r[i][3] = add2(r[i][3], bf16x2_to_f2(x[i].w));
+        q = fma2(r[i][3], r[i][3], fma2(r[i][2], r[i][2], fma2(r[i][1], r[i][1], fma2(r[i][0], r[i][0], q))));
+        if (p.r)
+          st_stream_u4(reinterpret_cast<uint4 *>(p.r + at) + lane + i * tpr,
+                       make_uint4(f2_to_bf16x2(r[i][0].x, r[i][0].y), f2_to_bf16x2(r[i][1].x, r[i][1].y), f2_to_bf16x2(r[i][2].x, r[i][2].y),
+                                  f2_to_bf16x2(r[i][3].x, r[i][3].y)));
       }
-      if (in && p.r)
-        st_stream_u4(reinterpret_cast<uint4 *>(p.r + (size_t)row * p.cols) + k,
-                     make_uint4(f2_to_bf16x2(r[i][0], r[i][1]), f2_to_bf16x2(r[i][2], r[i][3]), f2_to_bf16x2(r[i][4], r[i][5]), f2_to_bf16x2(r[i][6], r[i][7])));
     }
     if (!wb4) return;
-    const float yinv = 1.f / sqrtf(row_reduce<OpSum>(q, c, tpr, 1) / (float)p.cols + p.eps);
+    const float yinv = 1.f / sqrtf(row_sum(q.x + q.y, c, whole, 1) / (float)p.cols + p.eps);
+    const float2 yinv2 = make_float2(yinv, yinv);
 #pragma unroll
     for (int i = 0; i < kMaxVec; ++i) {
-      const int k = i * tpr + lane;
-      if (k < nv && live) {
-        const uint4 wv = __ldg(wb4 + k);
-        const uint32_t uw[4] = {wv.x, wv.y, wv.z, wv.w};
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 fw = bf16x2_to_f2(uw[j]);
-          o[j] = f2_to_bf16x2(r[i][2 * j] * yinv * fw.x, r[i][2 * j + 1] * yinv * fw.y);
-        }
-        st_stream_u4(reinterpret_cast<uint4 *>(p.y + (size_t)row * p.cols) + k, make_uint4(o[0], o[1], o[2], o[3]));
+      if (i * tpr < mine) {
+        const uint4 v = __ldg(wb4 + i * tpr);
+        const float2 f0 = mul2(mul2(r[i][0], yinv2), bf16x2_to_f2(v.x)), f1 = mul2(mul2(r[i][1], yinv2), bf16x2_to_f2(v.y));
+        const float2 f2 = mul2(mul2(r[i][2], yinv2), bf16x2_to_f2(v.z)), f3 = mul2(mul2(r[i][3], yinv2), bf16x2_to_f2(v.w));
+        st_stream_u4(reinterpret_cast<uint4 *>(p.y + at) + lane + i * tpr,
+                     make_uint4(f2_to_bf16x2(f0.x, f0.y), f2_to_bf16x2(f1.x, f1.y), f2_to_bf16x2(f2.x, f2.y), f2_to_bf16x2(f3.x, f3.y)));
       }
     }
   }

@@ -221,11 +221,15 @@ const char *residual_norm_problem(const bfuse_kernel_desc &d) {
   if (s[3] < 0) return "shape[3] (rows that share a row of the gate) must not be negative";
   return nullptr;
 }
-// Threads per row: the fewest, from 8, that leave a thread at most two vectors of 8 values, 256 at most.
-int residual_norm_threads(int cols) {
+// Threads per row: with many rows as few as hold it, four vectors of 8 values each (12000 rows of 4096 columns: 128 threads
+// 65 us, 256 threads 86), a power of two up to 32, then whole warps; with fewer rows than four per SM a thread per vector, up
+// to 256, for a row's latency is what counts (512 rows: 4.7 us against 5.2, one row 3.2 against 3.9).  Two rows and more per
+// CTA where they fill 256 threads (2048 rows of 4096: 11.7 us against 14.1).
+int residual_norm_threads(int rows, int cols, int sm) {
+  const int vecs = cols / 8, per = rows < 4 * sm ? 1 : 4;
   int tpr = 8;
-  while (tpr < 256 && cols > 16 * tpr) tpr *= 2;
-  return tpr;
+  while (tpr < 32 && tpr * 4 < vecs) tpr *= 2;
+  return tpr * 4 < vecs || (per == 1 && vecs > 32) ? std::min(256, round_up32(ceil_div(vecs, per))) : tpr;
 }
 
 // ---- attention: shape = seqs, total_q, total_kv, heads, kv heads, dim, q stride, kv stride, key slices ----
@@ -300,7 +304,7 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
     }
     case BFUSE_OP_RESIDUAL_NORM_BF16: {
       if (const char *m = residual_norm_problem(*d)) { *err = std::string("residual norm: ") + m; return BFUSE_ERR_SHAPE; }
-      const int tpr = residual_norm_threads(s[1]), rpc = std::max(1, 256 / tpr);
+      const int tpr = residual_norm_threads(s[0], s[1], sm), rpc = is_pow2(tpr) && (tpr <= 32 || s[0] >= 4 * sm) ? 256 / tpr : 1;
       set(ceil_div(s[0], rpc), 1, 1, tpr, rpc, 256, 6);
       return BFUSE_OK;
     }
@@ -732,7 +736,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
     case BFUSE_OP_RESIDUAL_NORM_BF16: {
       if (const char *m = residual_norm_problem(d)) return shape_err(m);
       const int tpr = kd.bx, rpc = kd.by;
-      if (!is_pow2(tpr) || kd.bz != 1) return shape_err("BlockDim must be (power-of-two threads per row, rows per CTA, 1)");
+      if ((!is_pow2(tpr) && rpc != 1) || kd.bz != 1) return shape_err("BlockDim must be (power-of-two threads per row, rows per CTA, 1), or (whole warps, 1, 1)");
       if (s[1] > 8 * ResidualNormBf16::kMaxVec * tpr) return shape_err("cols do not fit the per-thread vector budget");
       if (kd.gy != 1 || kd.gz != 1 || (long long)kd.gx * rpc < s[0]) return shape_err("GridDim.X * rows per CTA must cover the rows");
       if (tpr > 32 && k.smem < 256) return shape_err("rows wider than a warp need 256 bytes of shared memory");

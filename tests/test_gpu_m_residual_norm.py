@@ -51,7 +51,7 @@ def check(t, norms, gate_rows, scale):
 
 
 @pytest.mark.parametrize("cols", [8, 64, 264, 768, 1000, 2048, 4096, 5120, 8192])
-@pytest.mark.parametrize("rows", [1, 3, 130])
+@pytest.mark.parametrize("rows", [1, 3, 130, 700])
 def test_sizes(rt, rows, cols):
     import torch
     t, h = build(rt, rows, cols, 3, 0)
@@ -90,7 +90,7 @@ def test_in_place_stream(rt):
     assert (t["b"].double() - y).abs().max() <= 2.0 ** -7 * y.abs().max()
 
 
-@pytest.mark.parametrize("block", [(32, 8), (64, 1), (128, 2), (256, 1)])
+@pytest.mark.parametrize("block", [(32, 8), (64, 1), (96, 1), (160, 1), (128, 2), (256, 1)])
 def test_other_blocks(rt, block):
     import torch
     t, h = build(rt, 77, 1000, 3, 1, block=block)
