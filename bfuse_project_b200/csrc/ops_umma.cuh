@@ -231,6 +231,7 @@ struct GemmUmmaParams {
 // its tiles come and go in the same boxes.
 struct GemmActParams : GemmUmmaParams {
   alignas(64) CUtensorMap map_other;   // as map_out, for loads
+  const uint16_t *other;
   int has_other;                       // 0: no residual / gate
   int mul;                             // 1: act(...) * other, 0: act(...) + other
   int act;                             // BFUSE_ACT_*
@@ -248,19 +249,20 @@ __device__ __forceinline__ float activate(float x) {
   if (ACT == ACT_SILU) return over_one_plus_exp(x, x);
   return x;
 }
-__device__ __forceinline__ void activate16(int act, float (&v)[16]) {
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
   if (act == ACT_RELU) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_RELU>(v[j]);
+    for (int j = 0; j < N; ++j) v[j] = activate<ACT_RELU>(v[j]);
   } else if (act == ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_GELU>(v[j]);
+    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU>(v[j]);
   } else if (act == ACT_GELU_TANH) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_GELU_TANH>(v[j]);
+    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU_TANH>(v[j]);
   } else if (act == ACT_SILU) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = activate<ACT_SILU>(v[j]);
+    for (int j = 0; j < N; ++j) v[j] = activate<ACT_SILU>(v[j]);
   }
 }
 
@@ -408,6 +410,12 @@ struct ChunkWriter {
   }
 };
 
+// Few rows of A (tokens being decoded): multiplied the other way round, out^T = W A^T.  A stage then holds 128 rows of W and
+// only `bm` (16 or 32) of A instead of 128, so that eight stages are 128 KB of weights on their way per SM; the accumulator has
+// output columns in its lanes and rows in its columns, and what the k-slices exchange is 128 x bm.
+__host__ __device__ constexpr bool umma_few_rows(int bm) { return bm < kUmmaBM; }
+__host__ __device__ constexpr int umma_few_recv_bytes(int bm, int split) { return split > 1 ? kUmmaBM * bm * 4 : 0; }
+
 constexpr int kActBarOffset = 256;   // in the window's header: a barrier per epilogue warp and staging buffer
 constexpr int kActBars = 4;          // staging buffers of a warp at most (staging_plan: 64 bf16 columns a chunk, 256 a tile)
 
@@ -465,7 +473,7 @@ struct ActWriter : ChunkWriter<1> {
     v[4] += bb.x, v[5] += bb.y, v[6] += bb.z, v[7] += bb.w;
     v[8] += bc.x, v[9] += bc.y, v[10] += bc.z, v[11] += bc.w;
     v[12] += bd.x, v[13] += bd.y, v[14] += bd.z, v[15] += bd.w;
-    activate16(pa->act, v);
+    activate_all(pa->act, v);
     const uint32_t row = buf + (uint32_t)lane * 128u;
     if (pa->has_other) {
 #pragma unroll
@@ -626,7 +634,176 @@ struct GemmUmma {
     return true;
   }
 
+  // The tile of few rows: split (1, 2, 4 or 8) CTAs of a cluster, each a slice of K.  Every rank pushes its sums to the rank that
+  // owns the output column, into memory kept for that, so no one waits for the others' rings.
+  __device__ __forceinline__ static void run_few(const Params &p, const TileCtx &c) {
+    const int warp = c.tid >> 5, lane = c.tid & 31, quad = (threadIdx.x >> 5) & 3, at = quad * 32 + lane;   // at: output column of the tile
+    const int BM = p.bm, split = p.split, stages = p.stages, stage_bytes = umma_stage_bytes(kUmmaBM, BM);
+    const int kslice = c.block_x() % split, m0 = c.block_x() / split * BM, n0 = c.block_y() * kUmmaBM, bz = c.block_z();
+    const uint32_t full0 = smem_u32(c.smem), empty0 = full0 + 8 * kUmmaMaxStages, acc_bar = empty0 + 8 * kUmmaMaxStages, recv_bar = acc_bar + 8;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * (2 * kUmmaMaxStages + 2));
+    const uint32_t tiles = full0 + kUmmaHeaderBytes, recv = tiles + (uint32_t)(stages * stage_bytes);
+    const int cols = BM < 32 ? 32 : BM;
+    if (warp == 5 && !c.tmem_given) {
+      tmem_alloc(smem_u32(tmem_slot), cols);
+      if (!c.persistent) tmem_relinquish();
+    }
+    const int total_kb = (p.K + kBK - 1) / kBK, kb0 = kslice * p.kb_per_slice, num_kb = min(p.kb_per_slice, total_kb - kb0), npre = min(stages, num_kb);
+    auto load = [&](int kb, uint32_t s) {
+      const uint32_t dst = tiles + s * stage_bytes, bar = full0 + 8 * s;
+      mbar_expect_tx(bar, (uint32_t)stage_bytes);
+      tma_load_3d(dst + BM * kUmmaRowBytes, &p.map_b, bar, (kb0 + kb) * kBK, n0, bz);
+      tma_load_3d(dst, &p.map_a, bar, (kb0 + kb) * kBK, m0, bz);
+    };
+    if (warp == 4) {
+      if (lane < stages) {
+        mbar_init(full0 + 8 * lane, 1);
+        mbar_init(empty0 + 8 * lane, 1);
+      }
+      if (lane == 0) {
+        mbar_init(acc_bar, 1);
+        mbar_init(recv_bar, 1);
+      }
+      if (lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_a : &p.map_b) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      __syncwarp();
+      c.dependency_wait();
+      if (elect_one()) {
+        if (split > 1) mbar_expect_tx(recv_bar, (uint32_t)umma_few_recv_bytes(BM, split));
+        for (int kb = 0; kb < npre; ++kb) load(kb, (uint32_t)kb);
+      }
+      __syncwarp();
+    } else {
+      c.dependency_wait();
+    }
+    tc_fence_before();
+    c.sync();
+    tc_fence_after();
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA's barriers are up: its peers may push
+    const uint32_t tmem = c.tmem_given ? c.tmem_base : *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+    const int per = kUmmaBM / split;   // output columns a rank owns
+    bool ok = true;
+    if (warp == 4) {
+      if (elect_one()) {
+        uint32_t s = 0, ph = 0;
+        for (int kb = npre; kb < num_kb; ++kb) {
+          if (!mbar_wait(empty0 + 8 * s, ph, c.status, UMMA_WAIT_EMPTY_TIMEOUT)) break;
+          load(kb, s);
+          if (++s == (uint32_t)stages) s = 0, ph ^= 1;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 5) {
+      if (elect_one()) {
+        const uint32_t idesc = umma_idesc(KIND, BM), lo0 = ((tiles >> 4) & 0x3fffu) | (1u << 16), w_off = (uint32_t)(BM * kUmmaRowBytes) >> 4;
+        uint32_t s = 0, ph = 0, lo = lo0;
+        for (int kb = 0; kb < num_kb && ok; ++kb) {
+          ok = mbar_wait(full0 + 8 * s, ph, c.status, UMMA_WAIT_FULL_TIMEOUT);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma_ss<KIND>(tmem, lo + w_off + 2 * j, lo + 2 * j, idesc, kb > 0 || j > 0);
+          umma_commit(empty0 + 8 * s);
+          if (++s == (uint32_t)stages) s = 0, ph ^= 1, lo = lo0;
+          else lo += (uint32_t)stage_bytes >> 4;
+        }
+        umma_commit(acc_bar);
+        // (as in run(): no release may be in flight when the barriers go)
+        for (int kb = max(0, num_kb - stages); kb < num_kb && ok; ++kb)
+          ok = mbar_wait(empty0 + 8 * (kb % stages), (kb / stages) & 1, c.status, UMMA_WAIT_EMPTY_TIMEOUT);
+      }
+      __syncwarp();
+    }
+    // R sums of output column n, rows m, m + step ...: the loads of `other` first, then one after the other
+    const size_t batch_at = (size_t)bz * p.M * p.N;
+    auto finish = [&](auto &v, int m, int step, int n, float bias) {
+      constexpr int R = sizeof(v) / sizeof(v[0]);
+      const size_t i0 = batch_at + (size_t)m * p.N + n, next = (size_t)step * p.N;
+      float o[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        if (p.has_other && m + j * step < p.M) o[j] = __uint_as_float((uint32_t)__ldcg(p.other + i0 + j * next) << 16);
+#pragma unroll
+      for (int j = 0; j < R; ++j) v[j] += bias;
+      activate_all(p.act, v);
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        if (m + j * step < p.M) {
+          if (p.has_other) v[j] = p.mul ? v[j] * o[j] : v[j] + o[j];
+          reinterpret_cast<__nv_bfloat16 *>(p.out)[i0 + j * next] = __float2bfloat16_rn(v[j]);
+        }
+    };
+    auto ask_other = [&](int m, int n) {
+      if (p.has_other && m < p.M && n < p.N) prefetch_l2(p.other + batch_at + (size_t)m * p.N + n);
+    };
+    if (warp < 4) {
+      const int n = n0 + (split > 1 ? kslice * per + at % per : at), m_first = m0 + (split > 1 ? at / per : 0), m_step = split > 1 ? split : 1;
+      const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+      if ((at & 31) == 0 || split > 1)
+        for (int m = m_first; m < m0 + BM; m += m_step) ask_other(m, n);   // (one lane a line; with k-slices a warp's lanes are in several rows)
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_bar, 0, c.status, UMMA_WAIT_ACC_TIMEOUT));
+      tc_fence_after();
+      const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
+      if (split == 1) {
+#pragma unroll 1
+        for (int mb = 0; mb < BM && m0 + mb < p.M && ok; mb += 16) {
+          uint32_t r[16];
+          tmem_ld_32x16(trow + mb, r);
+          tmem_ld_wait();
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+          if (n < p.N) finish(v, m0 + mb, 1, n, bias);
+        }
+      } else {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const int owner = at / per;
+        const uint32_t dst = peer_smem(recv + (uint32_t)((kslice * per + at - owner * per) * BM) * 4, owner), bar = peer_smem(recv_bar, owner);
+#pragma unroll 1
+        for (int mb = 0; mb < BM; mb += 16) {
+          uint32_t r[16];
+          tmem_ld_32x16(trow + mb, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st_async_u4(dst + 4 * mb + 16 * j, bar, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(recv_bar, 0, c.status, UMMA_WAIT_PEERS_TIMEOUT)) && ok;
+        // (BM >= 16 and split <= 8: at least two rows a thread)
+        for (int m = m_first; m < min(m0 + BM, p.M) && ok && n < p.N; m += 2 * split) {
+          float v[2] = {0.f, 0.f};
+          for (int r = 0; r < split; ++r) {   // k-slice order
+            const uint32_t src = recv + (uint32_t)((r * per + at % per) * BM + m - m0) * 4;
+            v[0] += ld_shared_f32_at(src), v[1] += ld_shared_f32_at(src + 4 * split);
+          }
+          finish(v, m, split, n, bias);
+        }
+      }
+    } else if (split > 1) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    __syncwarp();
+    tc_fence_before();
+    c.sync();
+    if (warp == 5 && !c.tmem_given) tmem_dealloc(tmem, cols);
+    if (c.persistent && c.tid < stages) {
+      mbar_inval(full0 + 8 * c.tid);
+      mbar_inval(empty0 + 8 * c.tid);
+      if (c.tid == 0) {
+        mbar_inval(acc_bar);
+        mbar_inval(recv_bar);
+      }
+    }
+  }
+  __device__ __forceinline__ static float ld_shared_f32_at(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+  }
+
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
+    if constexpr (ACT) {
+      if (umma_few_rows(p.bm)) return run_few(p, c);
+    }
     const int warp = c.tid >> 5, lane = c.tid & 31;
     const int quad = (threadIdx.x >> 5) & 3;  // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
     const int BN = p.bn, BM = p.bm, halves = BM / kUmmaBM, kABytes = BM * kUmmaRowBytes, kStageBytes = umma_stage_bytes(BN, BM);

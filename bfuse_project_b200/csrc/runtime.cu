@@ -211,6 +211,21 @@ bool planes_pay(const int *s, int ohw, int tiles, int split, int share, int sm) 
 
 bool is_gemm_umma(int op) { return op == BFUSE_OP_GEMM_TF32 || op == BFUSE_OP_GEMM_BF16 || op == BFUSE_OP_GEMM_ACT_BF16; }
 
+// A GEMM_ACT of few rows runs transposed (GemmUmma::run_few): up to 32 rows by the runtime's choice, or where shape[6] asks for 16
+// or 32 (4 x 4096 x 14336: 22.5 us, 32.0 in tiles of 128 rows; 17 rows 25.9; 33 rows in tiles of 64 30.2, as in tiles of 128).
+// The k-slices: while every one finds an SM and keeps eight K blocks -- beside other operators 4 or none.
+bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
+  if (s[6] == 0 ? s[1] > 32 || (s[4] != 0 && s[4] != kUmmaBM) : (s[6] != 16 && s[6] != 32)) return false;
+  if (s[6] == 0) *bm = s[1] <= 16 ? 16 : 32;
+  if (s[5] > 0) return true;
+  const long long tiles = (long long)s[0] * ceil_div(s[1], *bm) * ceil_div(s[2], kUmmaBM) * share;
+  const int num_kb = ceil_div(s[3] * 2, kUmmaRowBytes);
+  *split = 1;
+  for (int c = share == 1 ? 8 : 4; c > 1 && *split == 1; c = share == 1 ? c / 2 : 1)
+    if (tiles * c <= sm && num_kb >= 8 * c) *split = c;
+  return true;
+}
+
 // ---- residual norm: shape = rows, cols, norms (BFUSE_NORM_*), rows that share a row of the gate (0: all) ----
 
 const char *residual_norm_problem(const bfuse_kernel_desc &d) {
@@ -430,6 +445,18 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0 || s[3] <= 0) { *err = "gemm: batch, M, N, K must be positive"; return BFUSE_ERR_SHAPE; }
       const int eb = d->op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
       int bn = s[4], split = s[5], bm = s[6], q;
+      if (d->op == BFUSE_OP_GEMM_ACT_BF16 && gemm_few_rows(s, share, sm, &bm, &split)) {
+        const int num_kb = ceil_div(s[3] * eb, kUmmaRowBytes);
+        if (split > num_kb || (split & (split - 1)) || split > 8) { *err = "gemm: a tile of few rows takes 1, 2, 4 or 8 k-slices, at most the number of K blocks"; return BFUSE_ERR_SHAPE; }
+        q = ceil_div(num_kb, split);
+        while ((split - 1) * q >= num_kb) split /= 2, q = ceil_div(num_kb, split);   // none empty
+        d->shape[4] = kUmmaBM, d->shape[5] = split, d->shape[6] = bm;
+        const long long ctas = (long long)split * s[0] * ceil_div(s[1], bm) * ceil_div(s[2], kUmmaBM);
+        const int budget = share * ctas <= sm ? 200 * 1024 : 110 * 1024, rest = kUmmaHeaderBytes + umma_few_recv_bytes(bm, split);
+        const int stages = std::min({q, kUmmaMaxStages, (budget - rest) / umma_stage_bytes(kUmmaBM, bm)});
+        set(split * ceil_div(s[1], bm), ceil_div(s[2], kUmmaBM), s[0], kUmmaThreads, 1, rest + stages * umma_stage_bytes(kUmmaBM, bm), 5);
+        return BFUSE_OK;
+      }
       if (bn <= 0 || split <= 0) pick_tile(s[0], s[1], s[2], s[3], eb, sm, share, bn, split, &bn, &split);
       if (bn != 32 && bn != 64 && bn != 128 && bn != 256) { *err = "gemm: BN must be 32, 64, 128 or 256"; return BFUSE_ERR_SHAPE; }
       d->shape[4] = bn;
@@ -796,11 +823,14 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       const int num_kb = ceil_div(s[3] * eb, kUmmaRowBytes), q = ceil_div(num_kb, split);
       if (split > 8 || (split - 1) * q >= num_kb) return shape_err("shape[5] (split) must be 1..8 with every k-slice non-empty");
       if (kd.bx != kUmmaThreads || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1)");
-      if ((bm != kUmmaBM && bm != 256) || (bm == 256 && split != 1) || bn * (bm / kUmmaBM) > 512)
-        return shape_err("shape[6] (BM) must be 128, or 256 with split = 1");
+      const bool few = act && (bm == 16 || bm == 32);   // few rows, transposed
+      if (few ? bn != kUmmaBM || (split & (split - 1)) != 0 : (bm != kUmmaBM && bm != 256) || (bm == 256 && split != 1) || bn * (bm / kUmmaBM) > 512)
+        return shape_err(act ? "shape[6] (BM) must be 128, or 256 with split = 1, or 16 or 32 with BN = 128 and 1, 2, 4 or 8 k-slices"
+                             : "shape[6] (BM) must be 128, or 256 with split = 1");
       if (kd.gx != split * ceil_div(s[1], bm) || kd.gy != ceil_div(s[2], bn) || kd.gz != s[0])
         return shape_err("GridDim must be (split * ceil(M/BM), ceil(N/BN), batch)");
-      if (k.smem < (size_t)umma_smem_bytes(bn, umma_min_stages(bn, split, eb, bm), bm))
+      const int rest = kUmmaHeaderBytes + (few ? umma_few_recv_bytes(bm, split) : 0);
+      if (k.smem < (size_t)(rest + (few ? 1 : umma_min_stages(bn, split, eb, bm)) * umma_stage_bytes(bn, bm)))
         return shape_err("shared memory below the store buffers (and, for a split GEMM, the receive area of the k-slices)");
       k.cluster = split;
       if (act && (d.flags & BFUSE_FLAG_CAUSAL)) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": no causal mask in this epilogue");
@@ -819,6 +849,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
         rc = encode_map(ctx, &p.map_other, eb, a[3], s[2], s[1], s[0], 32);
         if (rc) return rc;
         p.has_other = 1;
+        p.other = (const uint16_t *)a[3];
       }
       p.mul = act && (d.flags & BFUSE_FLAG_MUL) ? 1 : 0;
       p.act = act ? (int)((d.flags >> 4) & 15u) : 0;
@@ -826,7 +857,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       p.out = out;
       p.batch = s[0], p.M = s[1], p.N = s[2], p.K = s[3];
       p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL);
-      p.stages = std::min<int>(kUmmaMaxStages, (int)((k.smem - kUmmaHeaderBytes) / umma_stage_bytes(bn, bm)));
+      p.stages = std::min<int>(kUmmaMaxStages, (int)((k.smem - rest) / umma_stage_bytes(bn, bm)));
       p.bm = bm;
       p.bn = bn;
       p.split = split;
@@ -977,8 +1008,9 @@ bool ring_info(const KernelRec &k, int *header, int *stage_bytes, int *min_stage
   if (is_gemm_umma(k.desc.op)) {
     const int eb = k.desc.op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
     const int bm = s[6] > 0 ? s[6] : kUmmaBM;
-    *header = kUmmaHeaderBytes, *stage_bytes = umma_stage_bytes(s[4], bm);
-    *min_stages = umma_min_stages(s[4], std::max(1, s[5]), eb, bm);
+    const bool few = umma_few_rows(bm);
+    *header = kUmmaHeaderBytes + (few ? umma_few_recv_bytes(bm, s[5]) : 0), *stage_bytes = umma_stage_bytes(s[4], bm);
+    *min_stages = few ? 1 : umma_min_stages(s[4], std::max(1, s[5]), eb, bm);
     *stages = reinterpret_cast<const GemmUmmaParams *>(k.params)->stages;
     return true;
   }

@@ -74,6 +74,20 @@ def test_default_tilings(rt, m, n, k):
     run(rt, 1, m, n, k, bf.ACT_NONE, False, "add")
 
 
+@pytest.mark.parametrize("bm", [16, 32])
+@pytest.mark.parametrize("split", [1, 2, 4, 8])
+def test_few_rows(rt, bm, split):
+    for m in (1, bm - 1, bm, bm + 5):        # the last: two tiles
+        run(rt, 2, m, 264, 1096, bf.ACT_GELU, True, "add", tiling=(128, split, bm))
+    run(rt, 1, bm, 8, 1096, bf.ACT_SILU, False, "mul", tiling=(128, split, bm))
+
+
+@pytest.mark.parametrize("m", [1, 16, 17, 32, 33])
+def test_few_rows_with_long_k(rt, m):
+    run(rt, 1, m, 1024, 8192, bf.ACT_NONE, True, "add")
+    run(rt, 1, m, 136, 72, bf.ACT_RELU, True, None)
+
+
 def test_smallest_ring_reuses_its_buffers(rt):
     import torch
     t, h = build(rt, 1, 500, 512, 256, bf.ACT_RELU, True, "add", tiling=(256, 1, 256))
@@ -121,6 +135,24 @@ def test_fused_launches_give_the_same_bits(rt, pattern):
     assert rt.read_status() == 0
     check(torch, t1, bf.ACT_SILU, "mul")
     check(torch, t2, bf.ACT_GELU, "add")
+    want = [t1["out"].clone(), t2["out"].clone()]
+    t1["out"].zero_(), t2["out"].zero_()
+    rt.launch_fused(f, stream)
+    assert rt.read_status() == 0
+    assert torch.equal(t1["out"], want[0]) and torch.equal(t2["out"], want[1])
+
+
+@pytest.mark.parametrize("pattern", [bf.ZIGZAG, bf.PROPORTIONAL, bf.SM_STRIPED, bf.THREAD_SPLIT, bf.RANGE_SPLIT, bf.WORK_QUEUE])
+def test_fused_tiles_of_few_rows_give_the_same_bits(rt, pattern):
+    import torch
+    stream = torch.cuda.current_stream().cuda_stream
+    t1, a = build(rt, 1, 5, 1024, 4096, bf.ACT_SILU, False, "mul", share=2, seed=1)
+    t2, b = build(rt, 1, 30, 512, 2048, bf.ACT_NONE, True, "add", share=2, seed=2)
+    f = rt.register_fusion(a, b, pattern, 1, 1)
+    rt.launch_sequential(f, stream)
+    assert rt.read_status() == 0
+    check(torch, t1, bf.ACT_SILU, "mul")
+    check(torch, t2, bf.ACT_NONE, "add")
     want = [t1["out"].clone(), t2["out"].clone()]
     t1["out"].zero_(), t2["out"].zero_()
     rt.launch_fused(f, stream)
