@@ -46,7 +46,7 @@ struct PairEntry {
   ClusterCapFn mixed_clusters;
 };
 struct SingleEntry {
-  SingleLaunchFn launch, launch_other;   // launch_other: a conv staged as whole planes, attention with two tiles per CTA, else nullptr
+  SingleLaunchFn launch, launch_other;   // launch_other: a conv staged as whole planes, attention with two tiles per CTA, a GEMM of CTA pairs, else nullptr
   AttrFn attr;
   GroupLaunchFn group;       // up to kGroupMax operators of this body in one launch
   AttrFn group_attr;

@@ -1034,4 +1034,220 @@ struct GemmUmma {
   }
 };
 
+// ---- large products: pairs of CTAs that walk 256 x 256 tiles ----
+//
+// With a whole-SM tile per CTA the tensor pipe idles while the epilogue turns the accumulator into the output: 4096 x 14336 x
+// 4096 with SiLU and a gate took 480 us, 357 without any epilogue to speak of.  Here two CTAs of a cluster multiply a
+// 256 x 256 tile together (tcgen05 cta_group::2: each holds 128 rows of A, 128 rows of W and 128 rows of the accumulator, so
+// the operands cost no more L2 traffic per flop than a 256 x 256 tile on one SM), which leaves tensor memory for a second
+// accumulator: one tile's epilogue runs under the next one's MMAs.  A pair takes every pairs-th tile, rows of tiles
+// fastest; the rings go on across tiles.
+//
+// BlockDim = (192, 1, 1), warps as in GemmUmma; the MMAs are issued by the cluster's first CTA.  Every CTA loads its own
+// operands and reports them to the first one's barriers; a stage is given up, and an accumulator announced, in both.
+constexpr int kPairStages = 5, kPairBufs = 3;
+constexpr int kPairTile = 256;
+constexpr int kPairStageBytes = 2 * kUmmaABytes;   // 128 rows of A, 128 rows of W
+__host__ __device__ constexpr int pair_smem_bytes() { return kUmmaHeaderBytes + kPairStages * kPairStageBytes + kPairBufs * kUmmaStagingBytes; }
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives at the barrier at this address in both CTAs of the pair once the MMAs issued so far are done
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// As ActWriter, tile after tile through three buffers: the next chunk's `other` is on its way while this one is worked on.
+struct PairWriter : ActWriter {
+  int base = 0;   // chunks of the tiles before this one
+  __device__ __forceinline__ void load_chunk(int q) {
+    const uint32_t s = (uint32_t)(q % kPairBufs), bar = bar0 + 8 * s;
+    mbar_expect_tx(bar, 4096u);
+    tma_load_3d(buf0 + s * 4096u, &pa->map_other, bar, col0 + (q - base) * nb_step, m0, bz);
+  }
+  __device__ __forceinline__ uint32_t begin_chunk() {
+    if (lane == 0) {
+      tma_store_wait_read<1>();   // all but the last chunk's store have read their buffers: this one's and the next one's are free
+      if (pa->has_other) {
+        if (next >= loaded) load_chunk(next);
+        if (next + 1 < total) load_chunk(next + 1);
+      }
+    }
+    __syncwarp();
+    if (pa->has_other) {
+      loaded = min(next + 2, total);
+      mbar_wait(bar0 + 8 * (uint32_t)(next % kPairBufs), (next / kPairBufs) & 1, status, UMMA_WAIT_OTHER_TIMEOUT);
+      __syncwarp();
+    }
+    ++next;
+    return buf0 + (uint32_t)slot * 4096u;
+  }
+};
+
+struct GemmActPairs {
+  using Params = GemmActParams;
+  static constexpr int kMaxThreads = kUmmaThreads;
+  static constexpr int kMinBlocks = 1;
+  static constexpr bool kMemoryBound = false;
+  static constexpr bool kUsesTmem = true;
+  static constexpr int kBK = 64;
+
+  __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
+    const int warp = c.tid >> 5, lane = c.tid & 31, quad = (threadIdx.x >> 5) & 3;
+    const int rank = c.vblock & 1, pair = c.vblock >> 1, pairs = c.gx >> 1;
+    const int tiles_m = (p.M + kPairTile - 1) / kPairTile, tiles_n = (p.N + kPairTile - 1) / kPairTile, total = p.batch * tiles_m * tiles_n;
+    const int num_kb = (p.K + kBK - 1) / kBK;
+    const uint32_t full0 = smem_u32(c.smem), empty0 = full0 + 8 * kUmmaMaxStages, acc_full = empty0 + 8 * kUmmaMaxStages, acc_empty = acc_full + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * (2 * kUmmaMaxStages + 4));
+    float *bias_tile = reinterpret_cast<float *>(c.smem + 1024);
+    const uint32_t ring = full0 + kUmmaHeaderBytes, staging = ring + kPairStages * kPairStageBytes;
+    if (warp == 5) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (warp == 4) {
+      if (lane < kPairStages) {
+        mbar_init(full0 + 8 * lane, 1);
+        mbar_init(empty0 + 8 * lane, 1);
+      }
+      if (lane < 2) {
+        mbar_init(acc_full + 8 * lane, 1);
+        mbar_init(acc_empty + 8 * lane, 256);
+      }
+      if (lane < 4 * kActBars) mbar_init(full0 + kActBarOffset + 8 * lane, 1);
+      if (lane < 4) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_a : lane == 1 ? &p.map_b : lane == 2 ? &p.map_out : &p.map_other) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      __syncwarp();
+    }
+    c.dependency_wait();
+    tc_fence_before();
+    cluster_sync_all();   // both CTAs' barriers are up, both have their tensor memory
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+    // tile i of this pair: M tiles vary fastest, so that the pairs at work share their W
+    auto place = [&](int t, int &m0, int &n0, int &bz) {
+      m0 = t % tiles_m * kPairTile;
+      n0 = t / tiles_m % tiles_n * kPairTile;
+      bz = t / (tiles_m * tiles_n);
+    };
+    bool ok = true;
+    if (warp == 4) {
+      if (elect_one()) {
+        uint32_t s = 0, ph = 1;
+        for (int t = pair; t < total && ok; t += pairs) {
+          int m0, n0, bz;
+          place(t, m0, n0, bz);
+          m0 += rank * kUmmaBM, n0 += rank * kUmmaBM;
+          for (int kb = 0; kb < num_kb; ++kb) {
+            ok = mbar_wait(empty0 + 8 * s, ph, c.status, UMMA_WAIT_EMPTY_TIMEOUT);
+            if (!ok) break;
+            const uint32_t dst = ring + s * kPairStageBytes, bar = peer_smem(full0 + 8 * s, 0);
+            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * kPairStageBytes);
+            tma_load_3d_pair(dst, &p.map_a, bar, kb * kBK, m0, bz);
+            tma_load_3d_pair(dst + kUmmaABytes, &p.map_b, bar, kb * kBK, n0, bz);
+            if (++s == kPairStages) s = 0, ph ^= 1;
+          }
+        }
+        // the last release of every slot that was used: none may be in flight when this CTA ends
+        const int mine = total > pair ? (total - pair + pairs - 1) / pairs : 0;
+        const long long uses = (long long)mine * num_kb;
+        if (uses < kPairStages) s = 0, ph = 0;
+        for (int i = 0; i < kPairStages && i < uses && ok; ++i) {
+          ok = mbar_wait(empty0 + 8 * s, ph, c.status, UMMA_WAIT_EMPTY_TIMEOUT);
+          if (++s == kPairStages) s = 0, ph ^= 1;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 5) {
+      if (rank == 0 && elect_one()) {
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kPairTile >> 3) << 17) | ((uint32_t)(kPairTile >> 4) << 24);
+        const uint32_t lo0 = ((ring >> 4) & 0x3fffu) | (1u << 16);
+        uint32_t s = 0, ph = 0, lo = lo0;
+        int i = 0;
+        for (int t = pair; t < total && ok; t += pairs, ++i) {
+          const uint32_t acc = tmem + (uint32_t)(i & 1) * 256u;
+          ok = mbar_wait(acc_empty + 8 * (i & 1), ((i >> 1) & 1) ^ 1, c.status, UMMA_WAIT_ACC_TIMEOUT);
+          tc_fence_after();
+          for (int kb = 0; kb < num_kb && ok; ++kb) {
+            ok = mbar_wait(full0 + 8 * s, ph, c.status, UMMA_WAIT_FULL_TIMEOUT);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) umma_ss_pair(acc, lo + 2 * j, lo + (kUmmaABytes >> 4) + 2 * j, idesc, kb > 0 || j > 0);
+            umma_commit_pair(empty0 + 8 * s);
+            if (++s == kPairStages) s = 0, ph ^= 1, lo = lo0;
+            else lo += kPairStageBytes >> 4;
+          }
+          umma_commit_pair(acc_full + 8 * (i & 1));
+        }
+      }
+      __syncwarp();
+    } else {
+      PairWriter w{};
+      w.map_out = &p.map_out, w.M = p.M, w.N = p.N, w.causal = 0;
+      w.buf0 = staging + (uint32_t)(quad * kPairBufs) * 4096u;
+      w.nbuf = kPairBufs, w.lane = lane, w.nb_step = 64, w.group = 1;
+      w.pa = &p, w.bar0 = full0 + kActBarOffset + 8 * kActBars * quad, w.status = c.status, w.per_half = 4;
+      const uint32_t empty_at[2] = {peer_smem(acc_empty, 0), peer_smem(acc_empty + 8, 0)};
+      int i = 0;
+      for (int t = pair; t < total; t += pairs, ++i) {   // (to the end after a wait that gave up, too: the four warps meet in every tile)
+        int m0, n0, bz;
+        place(t, m0, n0, bz);
+        m0 += rank * kUmmaBM;
+        asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory");   // the last tile's bias has been read
+        for (int k = c.tid; k < kPairTile; k += 128) bias_tile[k] = (p.bias && n0 + k < p.N) ? __ldg(p.bias + n0 + k) : 0.f;
+        asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory");
+        w.m_base = w.m0 = m0 + quad * 32, w.bz = bz, w.n_tile0 = w.col0 = n0;
+        w.base = 4 * i, w.total = 4 * i + 4;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, c.status, UMMA_WAIT_ACC_TIMEOUT));
+        if (!ok) continue;
+        tc_fence_after();
+        const uint32_t trow = tmem + (uint32_t)(i & 1) * 256u + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          const uint32_t buf = w.begin_chunk();
+#pragma unroll
+          for (int sub = 0; sub < 4; sub += 2) {
+            uint32_t r0[16], r1[16];
+            tmem_ld_32x16(trow + (ch * 4 + sub) * 16, r0);
+            tmem_ld_32x16(trow + (ch * 4 + sub + 1) * 16, r1);
+            tmem_ld_wait();
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r0[j]);
+            w.put16(buf, sub, n0 + ch * 64, v, bias_tile);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r1[j]);
+            w.put16(buf, sub + 1, n0 + ch * 64, v, bias_tile);
+          }
+          w.end_chunk(buf, n0 + ch * 64);
+        }
+        tc_fence_before();
+        mbar_arrive_cluster(empty_at[i & 1]);   // this accumulator may be written again
+      }
+      w.finish();
+      w.drain();
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync_all();   // neither CTA's memory is read, or reported to, any more
+    tc_fence_after();
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+};
+
 }  // namespace bfuse

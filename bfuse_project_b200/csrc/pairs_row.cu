@@ -81,6 +81,7 @@ void fill_pair_row<BFUSE_ROW>(PairEntry *row, SingleEntry *single) {
     single->attr = &attr_single<A>;
     single->launch_other = nullptr;
     if constexpr (std::is_same<A, AttentionBf16>::value) single->launch_other = &launch_single<AttentionBf16Two>;
+    if constexpr (std::is_same<A, GemmUmma<1, true>>::value) single->launch_other = &launch_single<GemmActPairs>;
   }
   single->group = &launch_group<A>;
   single->group_attr = &attr_group<A>;

@@ -226,6 +226,13 @@ bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
   return true;
 }
 
+// Pairs of CTAs that walk 256 x 256 tiles (GemmActPairs): alone in its launch, where the runtime may choose the tiling
+bool gemm_pairs(const int *s, int share, int sm) {
+  if (s[7] != 0) return s[7] == 2;
+  const long long tiles = (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile);
+  return share == 1 && s[4] == 0 && s[5] == 0 && s[6] == 0 && sm >= 2 && tiles > sm / 4 && s[3] >= 512;
+}
+
 // ---- residual norm: shape = rows, cols, norms (BFUSE_NORM_*), rows that share a row of the gate (0: all) ----
 
 const char *residual_norm_problem(const bfuse_kernel_desc &d) {
@@ -455,7 +462,17 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
         const int budget = share * ctas <= sm ? 200 * 1024 : 110 * 1024, rest = kUmmaHeaderBytes + umma_few_recv_bytes(bm, split);
         const int stages = std::min({q, kUmmaMaxStages, (budget - rest) / umma_stage_bytes(kUmmaBM, bm)});
         set(split * ceil_div(s[1], bm), ceil_div(s[2], kUmmaBM), s[0], kUmmaThreads, 1, rest + stages * umma_stage_bytes(kUmmaBM, bm), 5);
+        d->shape[7] = 1;
         return BFUSE_OK;
+      }
+      if (d->op == BFUSE_OP_GEMM_ACT_BF16) {
+        if (gemm_pairs(s, share, sm)) {
+          const long long tiles = (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile);
+          d->shape[4] = kPairTile, d->shape[5] = 1, d->shape[6] = kPairTile, d->shape[7] = 2;
+          set(2 * (int)std::min<long long>(tiles, sm / 2), 1, 1, kUmmaThreads, 1, pair_smem_bytes(), 5);
+          return BFUSE_OK;
+        }
+        d->shape[7] = 1;
       }
       if (bn <= 0 || split <= 0) pick_tile(s[0], s[1], s[2], s[3], eb, sm, share, bn, split, &bn, &split);
       if (bn != 32 && bn != 64 && bn != 128 && bn != 256) { *err = "gemm: BN must be 32, 64, 128 or 256"; return BFUSE_ERR_SHAPE; }
@@ -820,6 +837,12 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if (bn * eb < 128) return shape_err("shape[4] (BN) must span at least 128 bytes of output (64 for bf16): stores leave in 128-byte chunks");
       if ((s[3] * eb) % 16) return shape_err("K rows must be a multiple of 16 bytes (TMA stride rule)");
       if ((s[2] * eb) % 16) return shape_err("N must make output rows a multiple of 16 bytes");
+      const bool pairs = act && s[7] == 2;
+      if (act && (s[7] < 0 || s[7] > 2)) return shape_err("shape[7] must be 1 (a CTA per tile) or 2 (pairs of CTAs that walk 256 x 256 tiles)");
+      if (pairs && (bn != kPairTile || bm != kPairTile || split != 1)) return shape_err("shape[7] = 2 (pairs of CTAs) takes 256 x 256 tiles and one k-slice");
+      if (pairs && (kd.gy != 1 || kd.gz != 1 || kd.gx % 2 || kd.gx / 2 > (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile)))
+        return shape_err("GridDim of pairs of CTAs must be (2 * pairs, 1, 1), no more pairs than 256 x 256 tiles");
+      if (pairs && k.smem < (size_t)pair_smem_bytes()) return shape_err("shared memory below the ring and the store buffers of a pair");
       const int num_kb = ceil_div(s[3] * eb, kUmmaRowBytes), q = ceil_div(num_kb, split);
       if (split > 8 || (split - 1) * q >= num_kb) return shape_err("shape[5] (split) must be 1..8 with every k-slice non-empty");
       if (kd.bx != kUmmaThreads || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1)");
@@ -827,20 +850,20 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if (few ? bn != kUmmaBM || (split & (split - 1)) != 0 : (bm != kUmmaBM && bm != 256) || (bm == 256 && split != 1) || bn * (bm / kUmmaBM) > 512)
         return shape_err(act ? "shape[6] (BM) must be 128, or 256 with split = 1, or 16 or 32 with BN = 128 and 1, 2, 4 or 8 k-slices"
                              : "shape[6] (BM) must be 128, or 256 with split = 1");
-      if (kd.gx != split * ceil_div(s[1], bm) || kd.gy != ceil_div(s[2], bn) || kd.gz != s[0])
+      if (!pairs && (kd.gx != split * ceil_div(s[1], bm) || kd.gy != ceil_div(s[2], bn) || kd.gz != s[0]))
         return shape_err("GridDim must be (split * ceil(M/BM), ceil(N/BN), batch)");
       const int rest = kUmmaHeaderBytes + (few ? umma_few_recv_bytes(bm, split) : 0);
       if (k.smem < (size_t)(rest + (few ? 1 : umma_min_stages(bn, split, eb, bm)) * umma_stage_bytes(bn, bm)))
         return shape_err("shared memory below the store buffers (and, for a split GEMM, the receive area of the k-slices)");
-      k.cluster = split;
+      k.cluster = pairs ? 2 : split;
       if (act && (d.flags & BFUSE_FLAG_CAUSAL)) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": no causal mask in this epilogue");
       if (act && ((d.flags >> 4) & 15u) > BFUSE_ACT_SILU) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": unknown activation");
       if (act && (d.flags & BFUSE_FLAG_MUL) && !a[3]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": BFUSE_FLAG_MUL without the factor");
       GemmActParams p;
       std::memset(&p, 0, sizeof(p));
-      int rc = encode_map(ctx, &p.map_a, eb, a[0], s[3], s[1], s[0], bm);
+      int rc = encode_map(ctx, &p.map_a, eb, a[0], s[3], s[1], s[0], pairs ? kUmmaBM : bm);
       if (rc) return rc;
-      rc = encode_map(ctx, &p.map_b, eb, a[1], s[3], s[2], s[0], bn);
+      rc = encode_map(ctx, &p.map_b, eb, a[1], s[3], s[2], s[0], pairs ? kUmmaBM : bn);
       if (rc) return rc;
       void *const out = a[act ? 4 : 3];
       rc = encode_map(ctx, &p.map_out, eb, out, s[2], s[1], s[0], 32);
@@ -967,9 +990,16 @@ bool takes_runs(const FusionRec &f) { return f.launch.per_cta[0] > 1 || f.launch
 // Is the kernel a conv staged as whole planes?
 bool whole_planes(const KernelRec &k) { return k.desc.op == BFUSE_OP_CONV2D_TF32 && reinterpret_cast<const ConvUmmaParams *>(k.params)->plane_imgs > 0; }
 
-// Is the kernel attention in a form that has an SM to itself (two tiles per CTA, or all of tensor memory)?  Shared launches take
-// it with one tile per CTA, 256 columns and one key slice.
-bool lone_attention(const KernelRec &k) { return k.desc.op == BFUSE_OP_ATTENTION_BF16 && reinterpret_cast<const AttentionParams *>(k.params)->tmem_cols > 256; }
+// Does the kernel have SMs to itself: attention with two tiles per CTA or all of tensor memory, a GEMM of CTA pairs?  Shared
+// launches take it in the form of a CTA per tile, with one k-slice.
+bool lone(const KernelRec &k) {
+  if (k.desc.op == BFUSE_OP_ATTENTION_BF16) return reinterpret_cast<const AttentionParams *>(k.params)->tmem_cols > 256;
+  return k.desc.op == BFUSE_OP_GEMM_ACT_BF16 && k.desc.shape[7] == 2;
+}
+// Is it launched by the second kernel of its operator?
+bool other_kernel(const KernelRec &k) {
+  return whole_planes(k) || (k.desc.op == BFUSE_OP_ATTENTION_BF16 && k.desc.shape[9] == 2) || (k.desc.op == BFUSE_OP_GEMM_ACT_BF16 && k.desc.shape[7] == 2);
+}
 
 DispatchTable single_table(const bfuse_context *ctx, const KernelRec &k) {
   DispatchTable t;
@@ -990,7 +1020,7 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
   const DispatchTable t = single_table(ctx, k);
   const size_t smem = k.smem + 1024;
   const SingleEntry &se = ctx->singles[k.desc.op];
-  cudaError_t e = (whole_planes(k) || (k.desc.op == BFUSE_OP_ATTENTION_BF16 && k.desc.shape[9] == 2) ? se.launch_other : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
+  cudaError_t e = (other_kernel(k) ? se.launch_other : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
   if (e != cudaSuccess) return fail_cuda(ctx, e, ("launch " + k.name).c_str());
   return BFUSE_OK;
 }
@@ -1059,6 +1089,7 @@ int add_unsplit(bfuse_context *ctx, int reg, bool gathered, int *slot) {
   const bool attention = orig.desc.op == BFUSE_OP_ATTENTION_BF16;
   alt->desc.shape[conv ? 10 : attention ? 8 : 5] = 1;
   if (attention) alt->desc.shape[9] = 1, alt->desc.flags &= ~(7u << 8);   // tiled to share an SM
+  if (orig.desc.op == BFUSE_OP_GEMM_ACT_BF16 && orig.desc.shape[7] == 2) alt->desc.shape[4] = 0, alt->desc.shape[7] = 1, alt->desc.flags &= ~(7u << 8);
   if (!conv && !attention) alt->desc.shape[6] = 0;   // tile height: the runtime's choice for the unsplit form
   if (gathered) alt->desc.shape[9] = 0, alt->desc.shape[11] = 2;
   alt->desc.KernelName = nullptr;
@@ -1317,13 +1348,13 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
     f->retiled[i] = true;
     return (int)BFUSE_OK;
   };
+  for (int i = 0; i < 2; ++i)
+    if (lone(**side[i]))
+      if (const int rc = retile(i, false)) return rc;
   if (pattern == PATTERN_THREAD_SPLIT || pattern == PATTERN_WORK_QUEUE)
     for (int i = 0; i < 2; ++i)
       if ((*side[i])->cluster > 1)
         if (const int rc = retile(i, false)) return rc;
-  for (int i = 0; i < 2; ++i)
-    if (lone_attention(**side[i]))
-      if (const int rc = retile(i, false)) return rc;
   // Thread split lays the two windows side by side; whole planes, whose window cannot go below four weight stages and
   // two raw slots (up to 98 KB), give way to the gathered form where the sum does not fit with the rings at their shallowest.
   if (pattern == PATTERN_THREAD_SPLIT) {
@@ -1515,9 +1546,9 @@ int bfuse_register_group(bfuse_context *ctx, const int *kernels, int n, int patt
   } undo{ctx};
   int narrow = 0, wide = 0;   // cluster widths above 1
   for (int i = 0; i < n; ++i)
-    if (ks[i]->cluster > 1) narrow = narrow ? std::min(narrow, ks[i]->cluster) : ks[i]->cluster, wide = std::max(wide, ks[i]->cluster);
+    if (ks[i]->cluster > 1 && !lone(*ks[i])) narrow = narrow ? std::min(narrow, ks[i]->cluster) : ks[i]->cluster, wide = std::max(wide, ks[i]->cluster);
   for (int i = 0; i < n; ++i) {
-    if (lone_attention(*ks[i]) || (narrow != wide && slices_optional(ctx, *ks[i]))) {
+    if (lone(*ks[i]) || (narrow != wide && slices_optional(ctx, *ks[i]))) {
       if (const int rc = add_unsplit(ctx, kernels[i], false, &undo.h[i])) return rc;
       g->ks[i] = undo.h[i];
       ks[i] = ctx->kernels[undo.h[i]].get();

@@ -18,7 +18,10 @@ def rt():
     return bf.Runtime(0)
 
 
-def build(rt, batch, m, n, k, act, bias, other, tiling=(0, 0, 0), seed=0, share=1, std=1.0):
+PAIRS = (256, 1, 256, 2)     # pairs of CTAs that walk 256 x 256 tiles
+
+
+def build(rt, batch, m, n, k, act, bias, other, tiling=(0, 0, 0), seed=0, share=1, std=1.0, grid=None):
     import torch
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -27,7 +30,7 @@ def build(rt, batch, m, n, k, act, bias, other, tiling=(0, 0, 0), seed=0, share=
          "other": mk(batch, m, n) if other else None, "out": torch.full((batch, m, n), 7.0, device="cuda", dtype=torch.bfloat16)}
     d = rt.describe("gemm_act", bf.OP_GEMM_ACT_BF16, (batch, m, n, k) + tuple(tiling),
                     [None if t[x] is None else t[x].data_ptr() for x in ("a", "w", "bias", "other", "out")],
-                    flags=bf.flag_share(share) | bf.flag_act(act) | (bf.FLAG_MUL if other == "mul" else 0))
+                    flags=bf.flag_share(share) | bf.flag_act(act) | (bf.FLAG_MUL if other == "mul" else 0), grid=grid)
     return t, rt.register_kernel(d)
 
 
@@ -72,6 +75,19 @@ def test_tilings(rt, bn, split, bm, m, n):
 def test_default_tilings(rt, m, n, k):
     run(rt, 1, m, n, k, bf.ACT_GELU_TANH, False, "mul")
     run(rt, 1, m, n, k, bf.ACT_NONE, False, "add")
+
+
+@pytest.mark.parametrize("m,n,k", [(256, 256, 64), (1, 8, 8), (300, 520, 72), (513, 264, 1096), (129, 2000, 320)])
+@pytest.mark.parametrize("other", [None, "add", "mul"])
+def test_pairs_of_ctas(rt, m, n, k, other):
+    run(rt, 2, m, n, k, bf.ACT_SILU, True, other, tiling=PAIRS)
+    run(rt, 2, m, n, k, bf.ACT_NONE, False, other, tiling=PAIRS, grid=(2, 1, 1))      # one pair takes all tiles
+
+
+def test_pairs_take_several_tiles(rt):
+    run(rt, 1, 2100, 2600, 712, bf.ACT_GELU, True, "add", tiling=PAIRS)               # 99 tiles
+    run(rt, 1, 2100, 2600, 712, bf.ACT_GELU, True, "add", tiling=PAIRS, grid=(26, 1, 1))
+    run(rt, 1, 2048, 4096, 1024, bf.ACT_SILU, False, "mul")                            # the runtime's choice
 
 
 @pytest.mark.parametrize("bm", [16, 32])
@@ -140,6 +156,30 @@ def test_fused_launches_give_the_same_bits(rt, pattern):
     rt.launch_fused(f, stream)
     assert rt.read_status() == 0
     assert torch.equal(t1["out"], want[0]) and torch.equal(t2["out"], want[1])
+
+
+@pytest.mark.parametrize("pattern", [bf.ZIGZAG, bf.THREAD_SPLIT, bf.WORK_QUEUE])
+def test_pairs_share_a_launch_in_another_form(rt, pattern):
+    import torch
+    stream = torch.cuda.current_stream().cuda_stream
+    t1, a = build(rt, 1, 600, 512, 1024, bf.ACT_SILU, False, "mul", seed=1, tiling=PAIRS)
+    t2, b = build(rt, 1, 100, 256, 512, bf.ACT_NONE, True, "add", seed=2, share=2, tiling=(128, 1, 128))
+    f = rt.register_fusion(a, b, pattern, 1, 1)
+    assert rt.fusion_info(f)["retiled_unsplit"][0]
+    rt.launch_fused(f, stream)
+    assert rt.read_status() == 0
+    check(torch, t1, bf.ACT_SILU, "mul")
+    check(torch, t2, bf.ACT_NONE, "add")
+    t1["out"].zero_()
+    rt.launch_kernel(a, stream)
+    assert rt.read_status() == 0
+    check(torch, t1, bf.ACT_SILU, "mul")
+    if pattern == bf.ZIGZAG:
+        g = rt.register_group([a, b], pattern, 1, 1)
+        t1["out"].zero_()
+        rt.launch_group(g, stream)
+        assert rt.read_status() == 0
+        check(torch, t1, bf.ACT_SILU, "mul")
 
 
 @pytest.mark.parametrize("pattern", [bf.ZIGZAG, bf.PROPORTIONAL, bf.SM_STRIPED, bf.THREAD_SPLIT, bf.RANGE_SPLIT, bf.WORK_QUEUE])
