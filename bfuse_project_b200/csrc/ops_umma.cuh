@@ -239,31 +239,59 @@ struct GemmActParams : GemmUmmaParams {
 
 enum GemmAct : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4 };
 
-// x / (1 + e^-z) in fp32; the quick quotient is good to 2 ulp (the output is rounded to bf16) and 0 where e^-z passes 2^126
-__device__ __forceinline__ float over_one_plus_exp(float x, float z) { return __fdividef(x, 1.f + exp2f(z * -1.4426950408889634f)); }
+// The activations, two values at a time and without branches: an epilogue has one warp per scheduler, and erff's two ways cost
+// 137 clocks a value where this takes about 20.
+__device__ __forceinline__ float rcp_approx(float x) {   // 1 ulp; 0 from 2^126 on
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x / (1 + 2^-z)
+__device__ __forceinline__ float2 over_one_plus_exp2(float2 x, float2 z) {
+  return mul2(x, make_float2(rcp_approx(1.f + exp2_approx(-z.x)), rcp_approx(1.f + exp2_approx(-z.y))));
+}
 template <int ACT>
-__device__ __forceinline__ float activate(float x) {
-  if (ACT == ACT_RELU) return x > 0.f ? x : (x != x ? x : 0.f);
-  if (ACT == ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  if (ACT == ACT_GELU_TANH) return over_one_plus_exp(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));   // 1/2 (1 + tanh u) = 1 / (1 + e^-2u)
-  if (ACT == ACT_SILU) return over_one_plus_exp(x, x);
+__device__ __forceinline__ float2 activate(float2 x) {
+  if (ACT == ACT_RELU) return make_float2(x.x > 0.f ? x.x : (x.x != x.x ? x.x : 0.f), x.y > 0.f ? x.y : (x.y != x.y ? x.y : 0.f));
+  if (ACT == ACT_SILU) return over_one_plus_exp2(x, mul2(x, make_float2(1.4426950408889634f, 1.4426950408889634f)));
+  if (ACT == ACT_GELU_TANH) {   // 1/2 (1 + tanh u) = 1 / (1 + e^-2u), u = sqrt(2 / pi) (x + 0.044715 x^3)
+    constexpr float a = 2.302208198f, b = 0.10294324f;   // 2 sqrt(2 / pi) log2(e), and 0.044715 times that
+    return over_one_plus_exp2(x, mul2(x, fma2(mul2(x, x), make_float2(b, b), make_float2(a, a))));
+  }
+  if (ACT == ACT_GELU) {
+    // x Phi(x) with erfc(u) = (a1 t + ... + a5 t^5) e^(-u^2), t = 1 / (1 + p u), for u = |x| / sqrt(2) >= 0: Abramowitz and
+    // Stegun 7.1.26, within 1.5e-7 of erfc; Phi(-|x|) is half of it
+    const float2 u = make_float2(fabsf(x.x) * 0.70710678f, fabsf(x.y) * 0.70710678f);
+    const float2 d = fma2(u, make_float2(0.3275911f, 0.3275911f), make_float2(1.f, 1.f)), t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    const float2 s = mul2(mul2(u, u), make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    float2 q = fma2(t, make_float2(0.5f * 1.061405429f, 0.5f * 1.061405429f), make_float2(0.5f * -1.453152027f, 0.5f * -1.453152027f));
+    q = fma2(t, q, make_float2(0.5f * 1.421413741f, 0.5f * 1.421413741f));
+    q = fma2(t, q, make_float2(0.5f * -0.284496736f, 0.5f * -0.284496736f));
+    q = fma2(t, q, make_float2(0.5f * 0.254829592f, 0.5f * 0.254829592f));
+    q = mul2(mul2(q, t), make_float2(exp2_approx(s.x), exp2_approx(s.y)));   // Phi(-|x|)
+    return make_float2(x.x * (x.x > 0.f ? 1.f - q.x : q.x), x.y * (x.y > 0.f ? 1.f - q.y : q.y));
+  }
   return x;
+}
+template <int ACT, int N>
+__device__ __forceinline__ void activate_each(float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 y = activate<ACT>(make_float2(v[j], v[j + 1]));
+    v[j] = y.x, v[j + 1] = y.y;
+  }
 }
 template <int N>
 __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
-  if (act == ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_RELU>(v[j]);
-  } else if (act == ACT_GELU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU>(v[j]);
-  } else if (act == ACT_GELU_TANH) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU_TANH>(v[j]);
-  } else if (act == ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_SILU>(v[j]);
-  }
+  if (act == ACT_RELU) activate_each<ACT_RELU>(v);
+  else if (act == ACT_GELU) activate_each<ACT_GELU>(v);
+  else if (act == ACT_GELU_TANH) activate_each<ACT_GELU_TANH>(v);
+  else if (act == ACT_SILU) activate_each<ACT_SILU>(v);
 }
 
 // marks of the diagnostic timeline (nanoseconds on the global timer), written by virtual block 0
