@@ -1016,7 +1016,21 @@ DispatchTable single_table(const bfuse_context *ctx, const KernelRec &k) {
   return t;
 }
 
+// A launch goes to the context's device, whichever is current (with the default stream it would go to that one, with buffers of
+// another); the caller's device is current again afterwards.
+struct OnDevice {
+  int was = -1;
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&was) == cudaSuccess && was != device) cudaSetDevice(device);
+    else was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) cudaSetDevice(was);
+  }
+};
+
 int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
+  const OnDevice on(ctx->device);
   const DispatchTable t = single_table(ctx, k);
   const size_t smem = k.smem + 1024;
   const SingleEntry &se = ctx->singles[k.desc.op];
@@ -1123,6 +1137,7 @@ int launch_fused_rec(bfuse_context *ctx, FusionRec &f, cudaStream_t s, const Dis
   PairLaunchFn fn = f.plan.table.kind == DISPATCH_THREADS ? pe.thread : f.plan.table.queue ? pe.queue : (f.wide ? pe.block_wide : pe.block);
   alignas(64) unsigned char pa[kParamsBytes], pb[kParamsBytes];
   DispatchTable with_switch;
+  const OnDevice on(ctx->device);
   if (ctx->no_pdl) {
     with_switch = table ? *table : f.launch;
     with_switch.no_pdl = 1;
@@ -1660,6 +1675,7 @@ int bfuse_launch_group(bfuse_context *ctx, int group, void *stream) {
     params[b][count[b]++] = params_with_stages(*ctx->kernels[g.ks[i]], g.stages[i], scratch[i]);
   }
   g.plan.table.no_pdl = ctx->no_pdl;
+  const OnDevice on(ctx->device);
   cudaError_t e;
   if (g.op_lo != g.op_hi)
     e = ctx->pairs[g.op_lo][g.op_hi].mixed(g.plan.table, params[0], count[0], params[1], count[1], (unsigned)g.plan.fused_grid,
@@ -2051,7 +2067,7 @@ static int copy_in(bfuse_context *ctx, KernelRec &k, void *const *host, cudaStre
 }
 static int copy_out(bfuse_context *ctx, KernelRec &k, void *const *host, cudaStream_t s) {
   for (int i = 0; i < k.nargs; ++i)
-    if (k.arg[i].is_output) {
+    if (k.arg[i].is_output && k.desc.args[i]) {   // (an optional output may be absent)
       if (!host[i]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": missing host output buffer");
       CK(cudaMemcpyAsync(host[i], k.desc.args[i], k.arg[i].bytes, cudaMemcpyDeviceToHost, s));
     }

@@ -33,8 +33,9 @@ OVERHEAD_US = 1.0
 PATTERNS = ("zigzag", "zigzag2", "range", "striped", "thread_split")
 MODEL_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "pairing_model.json")
 
-# operator body -> class (ids of include/bfuse_b200.h: 0..3 row-wise, 4 / 5 CUDA-core, 6 / 7 tcgen05 GEMM, 8 tcgen05 conv)
-BODY_CLASS = {0: "row", 1: "row", 2: "row", 3: "row", 4: "simt", 5: "simt", 6: "gemm", 7: "gemm", 8: "conv"}
+# operator body -> class (ids of include/bfuse_b200.h: 0..3 and 10 row-wise, 4 / 5 CUDA-core, 6, 7 and 9 tcgen05 GEMM, 8 tcgen05 conv;
+# attention, 11, counts as a GEMM: it was not among the fitted operators)
+BODY_CLASS = {0: "row", 1: "row", 2: "row", 3: "row", 4: "simt", 5: "simt", 6: "gemm", 7: "gemm", 8: "conv", 9: "gemm", 10: "row", 11: "gemm"}
 
 
 def ctas_per_sm(threads, smem_bytes, regs_per_thread=0):

@@ -19,14 +19,17 @@ tiled for the whole GPU); `run_fused` the scheduled one, its operators tiled for
 launch.  `run_unfused` launches the fused program's kernels one by one: same bodies, same tilings, so
 bit-identical results (the two tilings of an operator can differ in their k-slices, i.e. in the order
 of a sum).
-Element-wise glue of the models (ReLU / GELU / SiLU, batch-norm, reshapes and transposes) has no
-operator body here: buffers are reinterpreted in the layout the next operator wants, which keeps
-every operator's shape and the dependency structure of the layer, not its numerical function.
+In the segments of the reference's lists (BERT, the Llama projections, ResNet) element-wise glue (ReLU / GELU / SiLU,
+batch-norm, reshapes and transposes) is left out: buffers are reinterpreted in the layout the next operator wants, which
+keeps every operator's shape and the dependency structure of the layer, not its numerical function.  `llama_layer` is a
+whole decoder layer that computes what the model computes: its activations, gates and residual adds ride in the epilogues of
+GEMM_ACT_BF16 and in RESIDUAL_NORM_BF16, its attention is ATTENTION_BF16 over prompts packed one after another.
 """
 import math
 
-from . import (FLAG_CAUSAL, MODE_KERNEL1, OP_CONV2D_F32_SIMT, OP_CONV2D_TF32, OP_GEMM_BF16, OP_GEMM_TF32, OP_LAYERNORM_F32,
-               OP_RMSNORM_BF16, OP_ROPE_BF16, OP_SOFTMAX_F32, RANGE_SPLIT, SM_STRIPED, THREAD_SPLIT, ZIGZAG, BfuseError, flag_share, pairing)
+from . import (ACT_NONE, ACT_SILU, FLAG_CAUSAL, FLAG_MUL, MODE_KERNEL1, NORM_AFTER, NORM_BEFORE, OP_ATTENTION_BF16, OP_CONV2D_F32_SIMT, OP_CONV2D_TF32,
+               OP_GEMM_ACT_BF16, OP_GEMM_BF16, OP_GEMM_TF32, OP_LAYERNORM_F32, OP_RESIDUAL_NORM_BF16, OP_RMSNORM_BF16, OP_ROPE_BF16,
+               OP_SOFTMAX_F32, RANGE_SPLIT, SM_STRIPED, THREAD_SPLIT, ZIGZAG, BfuseError, flag_act, flag_share, pairing)
 
 # the pair-selection model's pattern names -> (pattern, M, N) of bfuse_register_fusion
 MODEL_PATTERNS = {"zigzag": (ZIGZAG, 1, 1), "zigzag2": (ZIGZAG, 1, 2), "range": (RANGE_SPLIT, 0, 0), "striped": (SM_STRIPED, 0, 0),
@@ -299,6 +302,21 @@ class _Builder:
     def rope(self, name, q, inv_freq, y, seq, heads, dim):
         self._add(name, OP_ROPE_BF16, (seq, heads, dim), [q, inv_freq, y], [q, inv_freq], [y])
 
+    def dense_act(self, name, x, w, y, M, N, K, act=ACT_NONE, bias=None, other=None, mul=False):
+        """y = act(x w^T + bias) + other, or * other"""
+        self._add(name, OP_GEMM_ACT_BF16, (1, M, N, K), [x, w, bias, other, y], [b for b in (x, w, bias, other) if b], [y],
+                  flags=flag_act(act) | (FLAG_MUL if mul else 0))
+
+    def residual_norm(self, name, x, block, w, r, y, rows, cols, after=False, gate=None, gate_rows=0, scale=1.0, eps=1e-5):
+        """r = x + scale * gate * block (normed, if `after`); y = norm of r: w holds the norms' weights in that order"""
+        norms = (NORM_AFTER if after else 0) | (NORM_BEFORE if y else 0)
+        self._add(name, OP_RESIDUAL_NORM_BF16, (rows, cols, norms, gate_rows), [x, block, gate, w, r, y], [b for b in (x, block, gate, w) if b],
+                  [b for b in (r, y) if b], fparam=(eps, scale))
+
+    def attention(self, name, q, k, v, cu, y, seqs, tokens, heads, kv_heads, dim, scale, causal=True):
+        self._add(name, OP_ATTENTION_BF16, (seqs, tokens, tokens, heads, kv_heads, dim), [q, k, v, cu, None, y], [q, k, v, cu], [y],
+                  fparam=(scale,), flags=FLAG_CAUSAL if causal else 0)
+
     def conv(self, name, x, w, y, n, ci, h, wd, co, k, stride, pad):
         self._add(name, OP_CONV2D_TF32, (n, ci, h, wd, co, k, k, stride, pad, 0, 0), [x, w, y], [x, w], [y])
 
@@ -375,6 +393,48 @@ def llama_layer_projections(rt, torch, seq=512, hidden=4096, kv=1024, heads=32, 
     b.dense("gate_proj", "hn", "wgate", None, "gate", seq, ffn, hidden, OP_GEMM_BF16)
     b.dense("up_proj", "hn", "wup", None, "up", seq, ffn, hidden, OP_GEMM_BF16)
     b.dense("down_proj", "gate", "wdown", None, "down", seq, hidden, ffn, OP_GEMM_BF16)
+    return b, b.ops
+
+
+def llama_layer(rt, torch, lens=(512,), hidden=4096, heads=32, kv_heads=8, ffn=14336, seed=0):
+    """A whole Llama-3-8B decoder layer in bf16 over prompts of `lens` tokens packed one after another: input norm, Q / K / V
+    projections, RoPE, causal attention of each prompt, output projection, residual add + norm, the gated feed-forward
+    (SiLU(gate) * up) and its residual add.  (RoPE counts positions along the packed rows: attention sees their differences.)"""
+    t = torch
+    b = _Builder(rt, torch, seed)
+    bf = None if rt is None else t.bfloat16
+    d, tokens = hidden // heads, sum(lens)
+    kv = kv_heads * d
+    b.tensor("x", (tokens, hidden), bf)
+    b.buf["wn1"] = (1.0 + 0.1 * b.tensor("wn1", (hidden,))).to(bf)
+    b.buf["wn2"] = (1.0 + 0.1 * b.tensor("wn2", (hidden,))).to(bf)
+    for n, width in (("q", hidden), ("k", kv), ("v", kv)):
+        b.tensor("w" + n, (width, hidden), bf, std=hidden ** -0.5)
+        b.tensor(n, (tokens, width), bf, zero=True)
+    b.tensor("wo", (hidden, hidden), bf, std=hidden ** -0.5)
+    for n in ("gate", "up"):
+        b.tensor("w" + n, (ffn, hidden), bf, std=hidden ** -0.5)
+    b.tensor("wdown", (hidden, ffn), bf, std=ffn ** -0.5)
+    for n, width in (("xn", hidden), ("q_rot", hidden), ("k_rot", kv), ("ctx", hidden), ("attn", hidden), ("h", hidden), ("hn", hidden), ("up", ffn),
+                     ("act", ffn), ("out", hidden)):
+        b.tensor(n, (tokens, width), bf, zero=True)
+    b.buf["inv_freq"] = _Shape((d // 2,)) if rt is None else (500000.0 ** (-t.arange(0, d, 2, device=b.dev, dtype=t.float32) / d)).contiguous()
+    ends = [0]
+    for n in lens:
+        ends.append(ends[-1] + n)
+    b.buf["cu"] = _Shape((len(ends),)) if rt is None else t.tensor(ends, device=b.dev, dtype=t.int32)
+    b.rmsnorm("input_norm", "x", "wn1", "xn", tokens, hidden)
+    b.dense("q_proj", "xn", "wq", None, "q", tokens, hidden, hidden, OP_GEMM_BF16)
+    b.dense("k_proj", "xn", "wk", None, "k", tokens, kv, hidden, OP_GEMM_BF16)
+    b.dense("v_proj", "xn", "wv", None, "v", tokens, kv, hidden, OP_GEMM_BF16)
+    b.rope("rope_q", "q", "inv_freq", "q_rot", tokens, heads, d)
+    b.rope("rope_k", "k", "inv_freq", "k_rot", tokens, kv_heads, d)
+    b.attention("attention", "q_rot", "k_rot", "v", "cu", "ctx", len(lens), tokens, heads, kv_heads, d, d ** -0.5)
+    b.dense("o_proj", "ctx", "wo", None, "attn", tokens, hidden, hidden, OP_GEMM_BF16)
+    b.residual_norm("post_norm", "x", "attn", "wn2", "h", "hn", tokens, hidden)
+    b.dense("up_proj", "hn", "wup", None, "up", tokens, ffn, hidden, OP_GEMM_BF16)
+    b.dense_act("gate_proj", "hn", "wgate", "act", tokens, ffn, hidden, ACT_SILU, other="up", mul=True)
+    b.dense_act("down_proj", "act", "wdown", "out", tokens, hidden, ffn, other="h")
     return b, b.ops
 
 

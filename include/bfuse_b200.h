@@ -59,20 +59,28 @@ enum {
                               /* (staged wherever it can be), which writes 1, 2 or 3 back; a kernel          */
                               /* registered with 0 is gathered, and so is one whose 3 was written back and   */
                               /* that comes with the gathered form's GridDim or a window only that form fits */
-  BFUSE_OP_GEMM_ACT_BF16 = 9, /* args: A, W, bias|NULL, other|NULL, out   shape: batch, M, N, K, tiling as GEMM_BF16;  */
-                              /* out = act(A W^T + bias) + other, or * other with BFUSE_FLAG_MUL; act: BFUSE_FLAG_ACT;  */
-                              /* A, W, other, out bf16 (other in out's shape; it may be out), bias fp32; accumulated,   */
-                              /* activated and added in fp32, rounded once                                              */
+  BFUSE_OP_GEMM_ACT_BF16 = 9, /* args: A, W, bias|NULL, other|NULL, out   shape: batch, M, N, K, then BN, k-slices, BM as  */
+                              /* GEMM_BF16;  out = act(A W^T + bias) + other, or * other with BFUSE_FLAG_MUL; act:      */
+                              /* BFUSE_FLAG_ACT;  A, W, other, out bf16 (other in out's shape; it may be out), bias     */
+                              /* fp32; accumulated, activated and added in fp32, rounded once.  BM = 16 or 32 (with     */
+                              /* BN = 128 and 1, 2, 4 or 8 k-slices): few rows, multiplied the other way round; the     */
+                              /* runtime's choice for up to 32 rows.  shape[7] = 2 (with BN = BM = 256 and one k-slice): */
+                              /* pairs of CTAs walk 256 x 256 tiles, GridDim (2 * pairs, 1, 1); 1: a CTA per tile; 0:   */
+                              /* pairs for a large product that runs alone (BFUSE_FLAG_SHARE(1)), written back.  A      */
+                              /* kernel of pairs is re-tiled for a launch that it shares (bfuse_fusion_info)            */
   BFUSE_OP_RESIDUAL_NORM_BF16 = 10, /* args: x, block, gate|NULL, w|NULL, r|NULL, y|NULL   fparam: eps, scale           */
                               /* shape: rows, cols (a multiple of 8, at most 8192), norms (a sum of BFUSE_NORM_*), rows */
                               /* that share a row of the gate (0: all do);  with N(v) = v / sqrt(mean(v^2) + eps):      */
                               /* b = block, or N(block) * w[after];  r = x + scale * gate * b;  y = N(r) * w[before].   */
                               /* w holds a row of cols for each norm there is, in that order; y goes with the second    */
-                              /* norm, r may be left out beside it; r or y may be x or block                            */
+                              /* norm, r may be left out beside it; r or y may be x or block.  BlockDim: threads per row */
+                              /* (a power of two) x rows, or any number of warps x 1                                     */
   BFUSE_OP_ATTENTION_BF16 = 11, /* args: q, k, v, cu_q, cu_kv|NULL, out   fparam: scale   flags: BFUSE_FLAG_CAUSAL      */
                               /* shape: seqs, total_q, total_kv, heads, kv_heads, dim (a multiple of 8, at most 128),   */
                               /* q token stride, k / v token stride (elements, multiples of 8; 0: dense), key slices    */
-                              /* per tile (1, 2, 4 or 8: a thread-block cluster joins them; 0: the runtime's choice).   */
+                              /* per tile (1, 2, 4 or 8: a thread-block cluster joins them; 0: the runtime's choice),   */
+                              /* tiles per CTA (1, or 2 that share the keys, with one slice; 0: the runtime's choice,   */
+                              /* 2 only for a kernel that runs alone, which is re-tiled for a launch that it shares).   */
                               /* q [total_q, heads, dim], k and v [total_kv, kv_heads, dim], out [total_q, heads, dim]  */
                               /* dense; query head h reads kv head h / (heads / kv_heads).  cu_q and cu_kv hold         */
                               /* seqs + 1 rising token offsets (int32, DEVICE memory, read at every launch; NULL: cu_q): */
@@ -80,7 +88,7 @@ enum {
                               /* none; rows outside every sequence are left as they were.  Causal: the last query sees  */
                               /* the last key, the one before all but it, and so on.  A query without keys gives zeros. */
                               /* Keys and values outside a sequence may hold anything; inside one, a masked key may be  */
-                              /* NaN or infinite, a masked value must be finite.  Offsets that fall or leave the        */
+                              /* NaN or infinite, a masked value must be finite.  out may not overlap the inputs.  Offsets that fall or leave the        */
                               /* tensors: their sequence is left out and bfuse_read_status says BFUSE_STATUS_BAD_OFFSETS */
   BFUSE_OP_COUNT = 12
 };
@@ -178,7 +186,9 @@ int bfuse_register_fusion(bfuse_context *ctx, int kernel1, int kernel2, int patt
  * consecutive blocks: shape[4] / shape[5] = virtual blocks a launched CTA of kernel 1 / 2 takes (1: none, a CTA a slot); shape[1] = CTAs of the launched kernel resident at once according to cudaOccupancyMaxActiveClusters,
  * which counts one CTA per SM for kernels that allocate tensor memory (0: not asked, thread split).
  * shape[2] / shape[3] = 1 when kernel 1 / 2 runs in this fusion with ONE k-slice although it was
- * registered with several, or gathered although it was staged as whole planes (a thread split whose
+ * registered with several, with a CTA per tile although it was registered to run alone (GEMM_ACT of CTA pairs, attention
+ * with two tiles per CTA or with all of tensor memory: the form of a kernel registered with BFUSE_FLAG_SHARE(1) whose
+ * window fills an SM), or gathered although it was staged as whole planes (a thread split whose
  * windows do not fit side by side otherwise); a conv whose k-slices only the whole-plane form brought gives them up
  * beside an operator of another cluster width, in groups too: BFUSE_PATTERN_THREAD_SPLIT and BFUSE_PATTERN_WORK_QUEUE cannot host
  * operators launched as thread-block clusters, so such an operator is re-tiled unsplit for the fusion
