@@ -59,9 +59,10 @@ enum AttnStatus : int {
 
 __host__ __device__ constexpr int attn_chunks(int dim) { return dim <= 64 ? 1 : 2; }   // 64-element chunks of a head
 __host__ __device__ constexpr int attn_tile_bytes(int dim) { return attn_chunks(dim) * kAttnChunkBytes; }
-// behind the ring, with key slices: what the ranks push to one another for a tile of few rows, (m, l) of 16 rows from each of 8
-// and 128 dims of 16 rows
-__host__ __device__ constexpr int attn_few_join_bytes(int split) { return split > 1 ? 8 * 16 * 8 + 128 * 16 * 4 : 0; }
+// behind the ring, with key slices: what the ranks push to one another for a tile of few rows, (m, l) of 16 rows from each of up
+// to 8 and 128 dims of 16 rows
+constexpr int kAttnFewStats = 8 * 16 * 8;
+__host__ __device__ constexpr int attn_few_join_bytes(int split) { return split > 1 ? kAttnFewStats + 128 * 16 * 4 : 0; }
 __host__ __device__ constexpr int attn_smem_bytes(int dim, int tiles, int stages, int split) {
   return kUmmaHeaderBytes + (tiles + stages) * attn_tile_bytes(dim) + attn_few_join_bytes(split);
 }
@@ -186,9 +187,10 @@ struct Attention {
       }
       int at = 0;   // first tile of this lane's sequence
       if (p.sort) {
+        const int len = qb - qa + (kb - ka);
         for (int i = 0; i < p.seqs; ++i) {
-          const int m = __shfl_sync(0xffffffffu, n, i);
-          if (m > n || (m == n && i < lane)) at += m;
+          const int m = __shfl_sync(0xffffffffu, n, i), other = __shfl_sync(0xffffffffu, len, i);
+          if (other > len || (other == len && i < lane)) at += m;
         }
       } else {
         int upto = n;
@@ -923,7 +925,7 @@ struct Attention {
     cluster_wait();
     if (!mine) return;
     const int dims = w.chunks * 64, per_log2 = log2_of(dims) - log2_of(split), per = 1 << per_log2;
-    const uint32_t stats = w.few_join, recv = stats + 1024u;
+    const uint32_t stats = w.few_join, recv = stats + kAttnFewStats;
     read_o();
     if (at < dims) {
       const int owner = at >> per_log2;

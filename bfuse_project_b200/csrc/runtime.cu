@@ -287,7 +287,8 @@ constexpr size_t kAttnHalfSm = 113 * 1024;   // above this window one CTA fits a
 int attention_min_stages(int dim, int split) { return std::max(2, ceil_div(attn_join_bytes(dim, split), attn_tile_bytes(dim)) - 1); }
 // Slices of a tile's keys: while every slice still finds an SM and keeps two blocks of the average sequence (one token each for
 // 16 sequences of up to 4096 keys, 8 kv heads: 30 us with one slice and a CTA an SM, 37 with two slices and two CTAs an SM,
-// whose rings are half as deep).  Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
+// whose rings are half as deep; 16 slices of one token over 32768 keys are slower than 8, 43 us against 32: clusters of 16 do not
+// all fit at once).  Beside other operators 1 or 4, so that any two operators the runtime tiled can share a launch.
 int attention_slices(const int *s, int share, int sm) {
   if (s[8] > 0) return s[8];
   const long long base = attention_tiles(s, 1) * s[4] * share, blocks = ceil_div(s[2], s[0] * kAttnKeys);

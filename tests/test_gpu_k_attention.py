@@ -109,6 +109,7 @@ def test_rows_without_keys_are_zero(rt):
 @pytest.mark.parametrize("dim", [64, 128])
 def test_key_slices(rt, slices, dim):
     run(rt, [1, 1, 3, 1], [5, 1500, 700, 1], 8, 2, dim, True, slices)
+    run(rt, [1, 2, 0], [4000, 129, 7], 32, 4, dim, True, slices)      # 8 and 16 rows
     run(rt, [70], [1030], 8, 2, dim, False, slices)
 
 
