@@ -111,11 +111,6 @@ __device__ __forceinline__ void umma_ts_bf16(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "r"(b_lo), "r"(kUmmaDescHi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 8-byte store into a peer's shared memory that also credits 8 bytes to the peer's mbarrier
 __device__ __forceinline__ void st_async_f2(uint32_t peer_addr, uint32_t peer_bar, float a, float b) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%2, %3}, [%1];" ::"r"(peer_addr), "r"(peer_bar),
@@ -159,8 +154,9 @@ struct Attention {
 
   // Tile number t of the batch (T = 2: pair of tiles) into *tile: sequence i has ceil(len_i / (T P)) of them, the last
   // positions first.  One warp.  Up to 32 sequences: one a lane, the longest first where `sort` (more tiles than run at
-  // once: a long sequence that starts late ends last); more: 256 a round, 8 a lane.
-  __device__ __forceinline__ static void find_tile(const Params &p, int t, int lane, AttnTile *tile, int *status) {
+  // once: a long sequence that starts late ends last); more: 256 a round, 8 a lane (the last of the `tiles` there may be looks
+  // at every sequence, so that bad offsets are seen even if no tile is theirs).
+  __device__ __forceinline__ static void find_tile(const Params &p, int t, int tiles, int lane, AttnTile *tile, int *status) {
     const int positions = T * p.positions;
     auto bad = [&] { atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS); };
     auto put = [&](int q0, int q_len, int kv0, int kv_end, int qt) {
@@ -235,7 +231,7 @@ struct Attention {
           at += n[i];
         }
         __syncwarp();
-        return;
+        if (t + 1 < tiles) return;
       }
       before += total;
     }
@@ -299,7 +295,7 @@ struct Attention {
     w.xch = w.full0 + 1024, w.q = w.full0 + kUmmaHeaderBytes;
     w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes, w.few_join = w.ring + stages * w.tile_bytes;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * kBars);
-    AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 256);
+    AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 512);
 
     if (warp == kIssuer && !c.tmem_given) {
       tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
@@ -312,11 +308,12 @@ struct Attention {
         mbar_init(w.full0 + 8 * lane, 1);
         mbar_init(w.empty0 + 8 * lane, 1);
       }
+      static_assert(kBars - 2 * kAttnMaxStages <= 32 && 8 * kBars + 4 <= 512, "one lane a barrier, and the header's room");
       if (lane < kBars - 2 * kAttnMaxStages) mbar_init(w.q_bar + 8 * lane, by_threads(w, lane) ? 128 : 1);
       if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_q : lane == 1 ? &p.map_k : &p.map_v) : "memory");
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       c.dependency_wait();
-      find_tile(p, c.block_y(), lane, tile_slot, c.status);
+      find_tile(p, c.block_y(), c.gy, lane, tile_slot, c.status);
       const AttnTile t = *tile_slot;
       const bool few = t.found && few_rows(p, t);
       const int active = t.found ? (sub_tile(p, t, 0).npos * p.group + 31) >> 5 : 0;   // quarters of the (first) tile that hold a row
@@ -448,9 +445,10 @@ struct Attention {
     return true;
   }
 
+  // The MMAs run in the order they are issued, and two tiles take turns, one's MMAs under the other's exponentials.
   // Where p has columns of its own (p_col), S of block j + 1 is made as soon as the threads have S of block j in their
-  // registers, under its exponentials; else after p V of block j, since the MMAs of one CTA run in the order they are issued.
-  // p V starts with the 64 keys whose p comes first.  Two tiles take turns, one's MMAs under the other's exponentials.
+  // registers; else p lies over S, and it follows p V of block j.  p V starts with the 64 keys whose p comes first.
+  // (Blocks as two halves of 64 keys that go round by themselves are no faster: prompts this long run at the power limit.)
   __device__ __forceinline__ static bool multiply(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int n, uint32_t tmem) {
     const uint32_t idesc = umma_idesc(1, w.chunks * 64) | (1u << 16), stages = (uint32_t)p.stages;
     int nx[2] = {n, 0};
@@ -476,13 +474,13 @@ struct Attention {
         if (first(j, x) && !mbar_wait(w.full0 + 8 * v.slot, v.phase, c.status, ATTN_WAIT_KV_TIMEOUT)) return false;
         const uint32_t pt = tmem + 256u * x + (uint32_t)p.p_col;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          if (!mbar_wait(w.p_bar + 16 * x + 8 * part, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(w.p_bar + 16 * x + 8 * half, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t step = (uint32_t)(4 * part + i);   // of 16 keys
-            umma_ts_bf16(tmem + 256u * x + 128, pt + 8 * step, v_lo + 128 * step, idesc, j > 0 || part + i > 0);
+            const uint32_t step = (uint32_t)(4 * half + i);   // of 16 keys
+            umma_ts_bf16(tmem + 256u * x + 128, pt + 8 * step, v_lo + 128 * step, idesc, j > 0 || half + i > 0);
           }
         }
         if (last(j, x)) umma_commit(w.empty0 + 8 * v.slot);
@@ -499,11 +497,6 @@ struct Attention {
   // (a whole warp gives up or goes on: what follows are warp-wide tensor-memory instructions)
   __device__ __forceinline__ static bool warp_wait(uint32_t bar, uint32_t parity, int *status, int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
-  }
-  __device__ __forceinline__ static float lds_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
   }
 
   // Values past the end of the sequence are the next one's, or whatever the buffer holds: p is 0 there, but 0 * NaN is not,
@@ -545,7 +538,7 @@ struct Attention {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 a = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, mc2);
-      a.x = ex2(a.x), a.y = ex2(a.y);
+      a.x = exp2_approx(a.x), a.y = exp2_approx(a.y);
       sum = add2(sum, a);
       q[i] = f2_to_bf16x2(a.x, a.y);   // the second product takes bf16: half a step of p, as of the output
     }
@@ -562,13 +555,14 @@ struct Attention {
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
     float m = -INFINITY, l = 0.f;   // the maximum the exponentials are taken against, and their sum
     bool ok = true;
+    const uint32_t s_bar = w.s_bar + 8 * x, p_bar = w.p_bar + 16 * x, pv_bar = w.pv_bar + 8 * x, c_bar = w.c_bar + 8 * x;
     if (!mine && warp < kProducer) {
       for (int j = 0; j < n && ok; ++j) {
-        ok = warp_wait(w.s_bar + 8 * x, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
-        if (p.p_col) mbar_arrive(w.c_bar + 8 * x);
-        if (p.p_col && j > 0 && ok) ok = warp_wait(w.pv_bar + 8 * x, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
-        mbar_arrive(w.p_bar + 16 * x);
-        mbar_arrive(w.p_bar + 16 * x + 8);
+        ok = warp_wait(s_bar, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        if (p.p_col) mbar_arrive(c_bar);
+        if (p.p_col && j > 0 && ok) ok = warp_wait(pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+        mbar_arrive(p_bar);
+        mbar_arrive(p_bar + 8);
       }
     }
     if (mine && n > 0) {
@@ -577,7 +571,7 @@ struct Attention {
 #pragma unroll 1
       for (int j = 0; j < n && ok; ++j) {
         const int key0 = (b0 + j) * kAttnKeys;
-        ok = warp_wait(w.s_bar + 8 * x, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        ok = warp_wait(s_bar, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
         if (!ok) break;
         tc_fence_after();
         uint32_t r[4][32];
@@ -586,19 +580,18 @@ struct Attention {
         tmem_ld_wait();
         if (p.p_col) {
           tc_fence_before();
-          mbar_arrive(w.c_bar + 8 * x);   // S may be overwritten
+          mbar_arrive(c_bar);   // S may be overwritten
         }
         const int seen = limit - key0;   // columns 0..seen of this block count
-        const bool masked = __any_sync(0xffffffffu, seen < kAttnKeys - 1);
-        const float mx = masked ? largest<true>(r, seen, m) : largest<false>(r, seen, m);
+        const float mx = __any_sync(0xffffffffu, seen < kAttnKeys - 1) ? largest<true>(r, seen, m) : largest<false>(r, seen, m);
         if (p.p_col && j > 0) {   // p's columns are free, and O is whole, once p V of block j - 1 is done
-          ok = warp_wait(w.pv_bar + 8 * x, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          ok = warp_wait(pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
           tc_fence_after();
         }
         // O follows a larger maximum only when that grew by more than 2^8: p stays below 2^8 and the sums in fp32 lose
         // nothing, and O mostly stays where it is.  (Without p_col s_bar stands for every MMA before it: block j - 1 is in O.)
         if (__any_sync(0xffffffffu, (mx - m) * sc > 8.f)) {
-          const float f = mx == -INFINITY ? 1.f : ex2((m - mx) * sc);
+          const float f = mx == -INFINITY ? 1.f : exp2_approx((m - mx) * sc);
           m = mx;
           l *= f;
           if (j > 0) {
@@ -616,15 +609,14 @@ struct Attention {
         const int have = t.kv_len - key0;
         if (have < kAttnKeys && ok) ok = clear_tail(p, c, w, j, have, row, active * 32);
         const float mc = m == -INFINITY ? 0.f : m * sc;
-        const uint32_t p_tmem = trow + (uint32_t)p.p_col;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          exponentials(p_tmem + 16 * g, r[g], sc, mc, sum);
+          exponentials(trow + (uint32_t)p.p_col + 16 * g, r[g], sc, mc, sum);
           if (g & 1) {
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(w.p_bar + 16 * x + 8 * (g >> 1));
+            mbar_arrive(p_bar + 8 * (g >> 1));
           }
         }
         l += sum.x + sum.y;
@@ -689,9 +681,9 @@ struct Attention {
     if (top == -INFINITY) top = 0.f;
     for (int r = 0; r < split; ++r) {
       const float2 s = ld_shared_f2(area + (uint32_t)(r * kAttnRows + row) * 8);
-      sum += s.y * ex2(s.x - top);
+      sum += s.y * exp2_approx(s.x - top);
     }
-    const float f = l == 0.f ? 0.f : ex2(mlog - top) / sum;
+    const float f = l == 0.f ? 0.f : exp2_approx(mlog - top) / sum;
     const int pieces = w.chunks * 4;   // of 16 columns
 #pragma unroll 1
     for (int ch = 0; ch < pieces; ++ch) {
@@ -867,7 +859,7 @@ struct Attention {
           quads_reduce<OpMax, R>(c, w, quad, lane, mx);
 #pragma unroll
           for (int i = 0; i < R; ++i) {
-            const float f = mx[i] == -INFINITY ? 1.f : ex2(m[i] - mx[i]);
+            const float f = mx[i] == -INFINITY ? 1.f : exp2_approx(m[i] - mx[i]);
             m[i] = mx[i];
             l[i] *= f;
             mx[i] = f;
@@ -886,7 +878,7 @@ struct Attention {
         const uint32_t pt = pt_smem(w, j) + (uint32_t)(at >> 6) * 2048u + (uint32_t)(at & 7) * 2u;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          const float e = ex2(s[i] - (m[i] == -INFINITY ? 0.f : m[i]));
+          const float e = exp2_approx(s[i] - (m[i] == -INFINITY ? 0.f : m[i]));
           l[i] += e;
           asm volatile("st.shared.u16 [%0], %1;" ::"r"(pt + (uint32_t)(i * 128 + ((((at & 63) >> 3) ^ (i & 7)) << 4))), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(e)))
                        : "memory");
@@ -944,12 +936,12 @@ struct Attention {
       if (top == -INFINITY) top = 0.f;
       for (int r = 0; r < split; ++r) {
         const float2 st = ld_shared_f2(stats + (uint32_t)(r * R + at) * 8);
-        sum += st.y * ex2(st.x - top);
+        sum += st.y * exp2_approx(st.x - top);
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       for (int r = 0; r < split; ++r) {
         const float2 st = ld_shared_f2(stats + (uint32_t)(r * R + at) * 8);
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.xch + (uint32_t)(r * R + at) * 4), "f"(st.y == 0.f ? 0.f : ex2(st.x - top) * inv) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.xch + (uint32_t)(r * R + at) * 4), "f"(st.y == 0.f ? 0.f : exp2_approx(st.x - top) * inv) : "memory");
       }
     }
     quads_sync(c);
@@ -958,8 +950,8 @@ struct Attention {
       const int row = i >> per_log2, d = i & (per - 1);
       float v = 0.f;
       for (int r = 0; r < split; ++r) {   // rank order: the sum is deterministic
-        const float f = lds_f32(w.xch + (uint32_t)(r * R + row) * 4);
-        if (f != 0.f) v = fmaf(f, lds_f32(recv + (uint32_t)((r * per + d) * R + row) * 4), v);
+        const float f = ld_shared_f32(w.xch + (uint32_t)(r * R + row) * 4);
+        if (f != 0.f) v = fmaf(f, ld_shared_f32(recv + (uint32_t)((r * per + d) * R + row) * 4), v);
       }
       if (slice * per + d < p.dim) reinterpret_cast<__nv_bfloat16 *>(out_row(p, t, head, row))[slice * per + d] = __float2bfloat16_rn(v);
     }

