@@ -635,6 +635,12 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
     if (!a[i] && !k.arg[i].optional) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": missing argument buffer");
     if (a[i] && !aligned16(a[i])) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": argument buffers must be 16-byte aligned");
   }
+  // do buffers i and j share bytes (`same`: may j be i, address for address?)
+  auto clash = [&](int i, int j, bool same = false) {
+    const auto x = reinterpret_cast<uintptr_t>(a[i]), y = reinterpret_cast<uintptr_t>(a[j]);
+    return x && y && !(same && x == y) && x < y + k.arg[j].bytes && y < x + k.arg[i].bytes;
+  };
+  auto overlap_err = [&](const char *m) { return fail(ctx, BFUSE_ERR_INVALID, k.name + ": " + m); };
   std::memset(k.params, 0, sizeof(k.params));
   k.cluster = 1;
   switch (d.op) {
@@ -788,6 +794,9 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       const bool after = s[2] & BFUSE_NORM_AFTER, before = s[2] & BFUSE_NORM_BEFORE;
       if (!before && a[5]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": y is the output of the norm before the next block, which shape[2] leaves out");
       if (!a[4] && !a[5]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": missing argument buffer");
+      for (int out = 4; out < 6; ++out)
+        if (clash(out, 0, true) || clash(out, 1, true) || clash(out, 2) || clash(out, 3) || clash(4, 5))
+          return overlap_err("an output overlaps the gate, the weights, the other output or part of an input");
       const uint16_t *w = (const uint16_t *)a[3];
       ResidualNormBf16::Params p{(const uint16_t *)a[0], (const uint16_t *)a[1], (const uint16_t *)a[2], after ? w : nullptr,
                                  before ? w + (after ? s[1] : 0) : nullptr, (uint16_t *)a[4], (uint16_t *)a[5], s[0], s[1],
@@ -803,6 +812,8 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
         return shape_err("GridDim must be (key slices * kv heads, (total_q + seqs * (P - 1)) / P, 1) with P = 128 / (heads / kv heads) positions a tile, twice that with two tiles per CTA");
       if (k.smem < (size_t)attn_smem_bytes(s[5], two, attention_min_stages(s[5], split), split))
         return shape_err("shared memory below the queries and two blocks of keys or values (and, with key slices, what they exchange)");
+      for (int in = 0; in < 5; ++in)
+        if (clash(5, in)) return overlap_err("the output overlaps an input");
       k.cluster = split;
       AttentionParams p;
       std::memset(&p, 0, sizeof(p));
@@ -860,6 +871,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if (act && (d.flags & BFUSE_FLAG_CAUSAL)) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": no causal mask in this epilogue");
       if (act && ((d.flags >> 4) & 15u) > BFUSE_ACT_SILU) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": unknown activation");
       if (act && (d.flags & BFUSE_FLAG_MUL) && !a[3]) return fail(ctx, BFUSE_ERR_INVALID, k.name + ": BFUSE_FLAG_MUL without the factor");
+      if (act && (clash(4, 0) || clash(4, 1) || clash(4, 2) || clash(4, 3, true))) return overlap_err("the output overlaps an input");
       GemmActParams p;
       std::memset(&p, 0, sizeof(p));
       int rc = encode_map(ctx, &p.map_a, eb, a[0], s[3], s[1], s[0], pairs ? kUmmaBM : bm);

@@ -62,7 +62,8 @@ enum {
   BFUSE_OP_GEMM_ACT_BF16 = 9, /* args: A, W, bias|NULL, other|NULL, out   shape: batch, M, N, K, then BN, k-slices, BM as  */
                               /* GEMM_BF16;  out = act(A W^T + bias) + other, or * other with BFUSE_FLAG_MUL; act:      */
                               /* BFUSE_FLAG_ACT;  A, W, other, out bf16 (other in out's shape; it may be out), bias     */
-                              /* fp32; accumulated, activated and added in fp32, rounded once.  BM = 16 or 32 (with     */
+                              /* fp32; accumulated, activated and added in fp32, rounded once; out may not overlap the  */
+                              /* inputs otherwise.  BM = 16 or 32 (with                                                 */
                               /* BN = 128 and 1, 2, 4 or 8 k-slices): few rows, multiplied the other way round; the     */
                               /* runtime's choice for up to 32 rows.  shape[7] = 2 (with BN = BM = 256 and one k-slice): */
                               /* pairs of CTAs walk 256 x 256 tiles, GridDim (2 * pairs, 1, 1); 1: a CTA per tile; 0:   */
@@ -88,8 +89,9 @@ enum {
                               /* none; rows outside every sequence are left as they were.  Causal: the last query sees  */
                               /* the last key, the one before all but it, and so on.  A query without keys gives zeros. */
                               /* Keys and values outside a sequence may hold anything; inside one, a masked key may be  */
-                              /* NaN or infinite, a masked value must be finite.  out may not overlap the inputs.  Offsets that fall or leave the        */
-                              /* tensors: their sequence is left out and bfuse_read_status says BFUSE_STATUS_BAD_OFFSETS */
+                              /* NaN or infinite, a masked value must be finite.  out may not overlap the inputs.       */
+                              /* Offsets that fall or leave the tensors (for keys: of a sequence with queries): their   */
+                              /* sequence is left out and bfuse_read_status says BFUSE_STATUS_BAD_OFFSETS               */
   BFUSE_OP_COUNT = 12
 };
 

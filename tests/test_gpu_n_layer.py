@@ -162,3 +162,45 @@ def test_registration_refusals():
     refused(2, attn, (1, 8, 8, 4, 4, 64), [p, p, p, p, p, p], fparam=(0.0,))
     assert rt.read_status() == 0
     rt.close()
+
+
+def test_overlapping_buffers_are_refused():
+    import torch
+    rt = bf.Runtime(0)
+    p = torch.zeros(1 << 16, device="cuda", dtype=torch.bfloat16).data_ptr()
+    at = lambda i: p + 8192 * i
+    gemm, norm, attn = bf.OP_GEMM_ACT_BF16, bf.OP_RESIDUAL_NORM_BF16, bf.OP_ATTENTION_BF16
+
+    def describe(op, shape, args, **kw):
+        return rt.describe("k", op, shape, args, **kw)
+
+    def refused(*a, **kw):
+        with pytest.raises(bf.BfuseError) as e:
+            rt.register_kernel(describe(*a, **kw))
+        assert e.value.code == 1 and "overlap" in str(e.value)
+
+    def taken(*a, **kw):
+        rt.unregister_kernel(rt.register_kernel(describe(*a, **kw)))
+
+    size = (1, 8, 8, 8)                                                                  # 128 bytes each
+    for i in range(3):                                                                   # out over A, W, bias; a part of the residual
+        args = [at(0), at(1), at(2), at(3), at(4)]
+        args[4] = args[i] + 16
+        refused(gemm, size, args)
+    refused(gemm, size, [at(0), at(1), at(2), at(3), at(3) + 64])
+    taken(gemm, size, [at(0), at(1), at(2), at(3), at(3)])
+    taken(gemm, size, [at(0), at(1), at(2), at(3), at(0) + 128])                          # behind A
+    size, kw = (4, 64, 3, 2), dict(fparam=(1e-5, 1.0))                                   # 512 bytes
+    refused(norm, size, [at(0), at(1), at(2), at(3), at(2), at(5)], **kw)                # the gate
+    refused(norm, size, [at(0), at(1), at(2), at(3), at(4), at(3) + 128], **kw)          # the weights
+    refused(norm, size, [at(0), at(1), at(2), at(3), at(4), at(4)], **kw)                # both outputs
+    refused(norm, size, [at(0), at(1), at(2), at(3), at(0) + 128, at(5)], **kw)          # other rows of the stream
+    taken(norm, size, [at(0), at(1), at(2), at(3), at(0), at(1)], **kw)
+    size, kw = (1, 8, 8, 1, 1, 64), dict(fparam=(0.1,))                                  # 1 KB
+    for i in range(5):
+        args = [at(0), at(1), at(2), at(3), at(4), at(5)]
+        args[5] = args[i]
+        refused(attn, size, args, **kw)
+    taken(attn, size, [at(0), at(1), at(2), at(3), at(4), at(0) + 1024], **kw)
+    assert rt.read_status() == 0
+    rt.close()
