@@ -532,14 +532,14 @@ struct Attention {
       }
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
   }
-  __device__ __forceinline__ static void exponentials(uint32_t p_tmem, const uint32_t (&r)[32], float sc, float mc, float2 &sum) {
+  __device__ __forceinline__ static void exponentials(uint32_t p_tmem, const uint32_t (&r)[32], float sc, float mc, float2 (&sum)[2]) {
     const float2 sc2 = make_float2(sc, sc), mc2 = make_float2(-mc, -mc);
     uint32_t q[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 a = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, mc2);
       a.x = exp2_approx(a.x), a.y = exp2_approx(a.y);
-      sum = add2(sum, a);
+      sum[i & 1] = add2(sum[i & 1], a);   // (two chains: one alone is 64 adds deep, and cost a tenth of a block of 64 dims)
       q[i] = f2_to_bf16x2(a.x, a.y);   // the second product takes bf16: half a step of p, as of the output
     }
     tmem_st_32x16(p_tmem, q);
@@ -609,7 +609,9 @@ struct Attention {
         const int have = t.kv_len - key0;
         if (have < kAttnKeys && ok) ok = clear_tail(p, c, w, j, have, row, active * 32);
         const float mc = m == -INFINITY ? 0.f : m * sc;
-        float2 sum = make_float2(0.f, 0.f);
+        float2 sum[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sum[i] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           exponentials(trow + (uint32_t)p.p_col + 16 * g, r[g], sc, mc, sum);
@@ -619,7 +621,8 @@ struct Attention {
             mbar_arrive(p_bar + 8 * (g >> 1));
           }
         }
-        l += sum.x + sum.y;
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
       }
       if (ok) ok = warp_wait(w.o_bar + 8 * x, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
       tc_fence_after();
