@@ -1061,21 +1061,25 @@ struct GemmUmma {
   }
 };
 
-// ---- large products: pairs of CTAs that walk 256 x 256 tiles ----
+// ---- large products: pairs of CTAs that walk tiles of 256 rows ----
 //
 // With a whole-SM tile per CTA the tensor pipe idles while the epilogue turns the accumulator into the output: 4096 x 14336 x
-// 4096 with SiLU and a gate took 480 us, 357 without any epilogue to speak of.  Here two CTAs of a cluster multiply a
+// 4096 with SiLU and a gate took 480 us, 357 without any epilogue to speak of; in pairs it takes 320 to 345.  Here two CTAs of a cluster multiply a
 // 256 x 256 tile together (tcgen05 cta_group::2: each holds 128 rows of A, 128 rows of W and 128 rows of the accumulator, so
-// the operands cost no more L2 traffic per flop than a 256 x 256 tile on one SM), which leaves tensor memory for a second
+// the operands cost no more traffic per flop than a 256 x 256 tile on one SM), which leaves tensor memory for a second
 // accumulator: one tile's epilogue runs under the next one's MMAs.  A pair takes every pairs-th tile, rows of tiles
 // fastest; the rings go on across tiles.
 //
 // BlockDim = (192, 1, 1), warps as in GemmUmma; the MMAs are issued by the cluster's first CTA.  Every CTA loads its own
 // operands and reports them to the first one's barriers; a stage is given up, and an accumulator announced, in both.
-constexpr int kPairStages = 5, kPairBufs = 3;
-constexpr int kPairTile = 256;
-constexpr int kPairStageBytes = 2 * kUmmaABytes;   // 128 rows of A, 128 rows of W
-__host__ __device__ constexpr int pair_smem_bytes() { return kUmmaHeaderBytes + kPairStages * kPairStageBytes + kPairBufs * kUmmaStagingBytes; }
+//
+// What bounds them: a K block of a 256 x 256 tile passes through each SM's shared memory as 32 KB written and 48 KB read, 640
+// clocks at 128 bytes a clock, its MMAs take 512 (and large products the power the device may draw).  A tile of 256 x 128
+// takes 56 KB a K block, 437 clocks, for 256 of MMAs: for products of few tiles, which then spread over twice the SMs.
+constexpr int kPairRows = 256, kPairBufs = 3;
+__host__ __device__ constexpr int pair_stages(int bn) { return bn == 256 ? 5 : 7; }
+__host__ __device__ constexpr int pair_stage_bytes(int bn) { return kUmmaABytes + bn / 2 * kUmmaRowBytes; }   // 128 rows of A, half of W's
+__host__ __device__ constexpr int pair_smem_bytes(int bn) { return kUmmaHeaderBytes + pair_stages(bn) * pair_stage_bytes(bn) + kPairBufs * kUmmaStagingBytes; }
 
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int c0, int c1, int c2) {
   asm volatile(
@@ -1136,18 +1140,19 @@ struct GemmActPairs {
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
     const int warp = c.tid >> 5, lane = c.tid & 31, quad = (threadIdx.x >> 5) & 3;
     const int rank = c.vblock & 1, pair = c.vblock >> 1, pairs = c.gx >> 1;
-    const int tiles_m = (p.M + kPairTile - 1) / kPairTile, tiles_n = (p.N + kPairTile - 1) / kPairTile, total = p.batch * tiles_m * tiles_n;
+    const int BN = p.bn, stages = p.stages, stage_bytes = pair_stage_bytes(BN);
+    const int tiles_m = (p.M + kPairRows - 1) / kPairRows, tiles_n = (p.N + BN - 1) / BN, total = p.batch * tiles_m * tiles_n;
     const int num_kb = (p.K + kBK - 1) / kBK;
     const uint32_t full0 = smem_u32(c.smem), empty0 = full0 + 8 * kUmmaMaxStages, acc_full = empty0 + 8 * kUmmaMaxStages, acc_empty = acc_full + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * (2 * kUmmaMaxStages + 4));
     float *bias_tile = reinterpret_cast<float *>(c.smem + 1024);
-    const uint32_t ring = full0 + kUmmaHeaderBytes, staging = ring + kPairStages * kPairStageBytes;
+    const uint32_t ring = full0 + kUmmaHeaderBytes, staging = ring + (uint32_t)(stages * stage_bytes);
     if (warp == 5) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     if (warp == 4) {
-      if (lane < kPairStages) {
+      if (lane < stages) {
         mbar_init(full0 + 8 * lane, 1);
         mbar_init(empty0 + 8 * lane, 1);
       }
@@ -1167,8 +1172,8 @@ struct GemmActPairs {
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
     // tile i of this pair: M tiles vary fastest, so that the pairs at work share their W
     auto place = [&](int t, int &m0, int &n0, int &bz) {
-      m0 = t % tiles_m * kPairTile;
-      n0 = t / tiles_m % tiles_n * kPairTile;
+      m0 = t % tiles_m * kPairRows;
+      n0 = t / tiles_m % tiles_n * BN;
       bz = t / (tiles_m * tiles_n);
     };
     bool ok = true;
@@ -1178,30 +1183,30 @@ struct GemmActPairs {
         for (int t = pair; t < total && ok; t += pairs) {
           int m0, n0, bz;
           place(t, m0, n0, bz);
-          m0 += rank * kUmmaBM, n0 += rank * kUmmaBM;
+          m0 += rank * kUmmaBM, n0 += rank * (BN / 2);
           for (int kb = 0; kb < num_kb; ++kb) {
             ok = mbar_wait(empty0 + 8 * s, ph, c.status, UMMA_WAIT_EMPTY_TIMEOUT);
             if (!ok) break;
-            const uint32_t dst = ring + s * kPairStageBytes, bar = peer_smem(full0 + 8 * s, 0);
-            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * kPairStageBytes);
+            const uint32_t dst = ring + s * (uint32_t)stage_bytes, bar = peer_smem(full0 + 8 * s, 0);
+            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2u * (uint32_t)stage_bytes);
             tma_load_3d_pair(dst, &p.map_a, bar, kb * kBK, m0, bz);
             tma_load_3d_pair(dst + kUmmaABytes, &p.map_b, bar, kb * kBK, n0, bz);
-            if (++s == kPairStages) s = 0, ph ^= 1;
+            if (++s == (uint32_t)stages) s = 0, ph ^= 1;
           }
         }
         // the last release of every slot that was used: none may be in flight when this CTA ends
         const int mine = total > pair ? (total - pair + pairs - 1) / pairs : 0;
         const long long uses = (long long)mine * num_kb;
-        if (uses < kPairStages) s = 0, ph = 0;
-        for (int i = 0; i < kPairStages && i < uses && ok; ++i) {
+        if (uses < stages) s = 0, ph = 0;
+        for (int i = 0; i < stages && i < uses && ok; ++i) {
           ok = mbar_wait(empty0 + 8 * s, ph, c.status, UMMA_WAIT_EMPTY_TIMEOUT);
-          if (++s == kPairStages) s = 0, ph ^= 1;
+          if (++s == (uint32_t)stages) s = 0, ph ^= 1;
         }
       }
       __syncwarp();
     } else if (warp == 5) {
       if (rank == 0 && elect_one()) {
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kPairTile >> 3) << 17) | ((uint32_t)(kPairTile >> 4) << 24);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kPairRows >> 4) << 24);
         const uint32_t lo0 = ((ring >> 4) & 0x3fffu) | (1u << 16);
         uint32_t s = 0, ph = 0, lo = lo0;
         int i = 0;
@@ -1216,8 +1221,8 @@ struct GemmActPairs {
 #pragma unroll
             for (int j = 0; j < 4; ++j) umma_ss_pair(acc, lo + 2 * j, lo + (kUmmaABytes >> 4) + 2 * j, idesc, kb > 0 || j > 0);
             umma_commit_pair(empty0 + 8 * s);
-            if (++s == kPairStages) s = 0, ph ^= 1, lo = lo0;
-            else lo += kPairStageBytes >> 4;
+            if (++s == (uint32_t)stages) s = 0, ph ^= 1, lo = lo0;
+            else lo += (uint32_t)stage_bytes >> 4;
           }
           umma_commit_pair(acc_full + 8 * (i & 1));
         }
@@ -1225,10 +1230,11 @@ struct GemmActPairs {
       __syncwarp();
     } else {
       PairWriter w{};
+      const int chunks = BN / 64;
       w.map_out = &p.map_out, w.M = p.M, w.N = p.N, w.causal = 0;
       w.buf0 = staging + (uint32_t)(quad * kPairBufs) * 4096u;
       w.nbuf = kPairBufs, w.lane = lane, w.nb_step = 64, w.group = 1;
-      w.pa = &p, w.bar0 = full0 + kActBarOffset + 8 * kActBars * quad, w.status = c.status, w.per_half = 4;
+      w.pa = &p, w.bar0 = full0 + kActBarOffset + 8 * kActBars * quad, w.status = c.status, w.per_half = chunks;
       const uint32_t empty_at[2] = {peer_smem(acc_empty, 0), peer_smem(acc_empty + 8, 0)};
       int i = 0;
       for (int t = pair; t < total; t += pairs, ++i) {   // (to the end after a wait that gave up, too: the four warps meet in every tile)
@@ -1236,16 +1242,16 @@ struct GemmActPairs {
         place(t, m0, n0, bz);
         m0 += rank * kUmmaBM;
         asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory");   // the last tile's bias has been read
-        for (int k = c.tid; k < kPairTile; k += 128) bias_tile[k] = (p.bias && n0 + k < p.N) ? __ldg(p.bias + n0 + k) : 0.f;
+        for (int k = c.tid; k < BN; k += 128) bias_tile[k] = (p.bias && n0 + k < p.N) ? __ldg(p.bias + n0 + k) : 0.f;
         asm volatile("bar.sync %0, 128;" ::"r"(c.bar_id + 8) : "memory");
         w.m_base = w.m0 = m0 + quad * 32, w.bz = bz, w.n_tile0 = w.col0 = n0;
-        w.base = 4 * i, w.total = 4 * i + 4;
+        w.base = chunks * i, w.total = chunks * (i + 1);
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, c.status, UMMA_WAIT_ACC_TIMEOUT));
         if (!ok) continue;
         tc_fence_after();
         const uint32_t trow = tmem + (uint32_t)(i & 1) * 256u + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
-        for (int ch = 0; ch < 4; ++ch) {
+        for (int ch = 0; ch < chunks; ++ch) {
           const uint32_t buf = w.begin_chunk();
 #pragma unroll
           for (int sub = 0; sub < 4; sub += 2) {

@@ -226,11 +226,23 @@ bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
   return true;
 }
 
-// Pairs of CTAs that walk 256 x 256 tiles (GemmActPairs): alone in its launch, where the runtime may choose the tiling
-bool gemm_pairs(const int *s, int share, int sm) {
+long long gemm_pair_tiles(const int *s, int bn) { return (long long)s[0] * ceil_div(s[1], kPairRows) * ceil_div(s[2], bn); }
+// Pairs of CTAs that walk tiles of 256 rows and *bn columns (GemmActPairs): alone in its launch, where the runtime may choose the
+// tiling.  What a K block costs an SM, as measured: 15 in a 256 x 256 tile (0.28 us), 9 in a 256 x 128 one, 10 in a 128 x 128
+// tile of its own -- every operand is written to shared memory and read from there, and that sets the pace -- and the last
+// wide tile's epilogue, which no MMA covers, as much as 8 K blocks.  (us, wide / narrow / a CTA per tile: 512 x 4096 x 4096
+// 28.5 / 19.4 / 20.6, 1024 x 4096 x 4096 29.9 / 32.1 / 35.7, 1500 x 4096 x 4096 49.0 / 44.5 / 57.7, 2048 x 2048 x 2048 19.4 /
+// 17.9 / 19.5, 300 x 6000 x 2048 23.0 / 21.2 / 14.1.)  Not for fewer tiles than half the pairs: 256 x 4096 x 4096 17.0, 15.5 in
+// tiles of 64 columns.
+bool gemm_pairs(const int *s, int share, int sm, int *bn) {
+  const long long slots = std::max(1, sm / 2), kb = ceil_div(s[3], GemmActPairs::kBK);
+  const long long wide = (15 * ((gemm_pair_tiles(s, 256) + slots - 1) / slots)) * kb + 15 * 8;
+  const long long narrow = 9 * ((gemm_pair_tiles(s, 128) + slots - 1) / slots) * kb;
+  const long long single = 10 * (((long long)s[0] * ceil_div(s[1], kUmmaBM) * ceil_div(s[2], 128) + sm - 1) / sm) * kb;
+  *bn = s[7] == 2 && s[4] != 0 ? s[4] : wide <= narrow ? 256 : 128;
   if (s[7] != 0) return s[7] == 2;
-  const long long tiles = (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile);
-  return share == 1 && s[4] == 0 && s[5] == 0 && s[6] == 0 && sm >= 2 && tiles > sm / 4 && s[3] >= 512;
+  return share == 1 && s[4] == 0 && s[5] == 0 && s[6] == 0 && sm >= 2 && s[3] >= 512 && gemm_pair_tiles(s, *bn) > slots / 2 &&
+         std::min(wide, narrow) <= single;
 }
 
 // ---- residual norm: shape = rows, cols, norms (BFUSE_NORM_*), rows that share a row of the gate (0: all) ----
@@ -467,10 +479,11 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
         return BFUSE_OK;
       }
       if (d->op == BFUSE_OP_GEMM_ACT_BF16) {
-        if (gemm_pairs(s, share, sm)) {
-          const long long tiles = (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile);
-          d->shape[4] = kPairTile, d->shape[5] = 1, d->shape[6] = kPairTile, d->shape[7] = 2;
-          set(2 * (int)std::min<long long>(tiles, sm / 2), 1, 1, kUmmaThreads, 1, pair_smem_bytes(), 5);
+        if (int wide; gemm_pairs(s, share, sm, &wide)) {
+          if (wide != 128 && wide != 256) { *err = "gemm: pairs of CTAs take BN = 128 or 256"; return BFUSE_ERR_SHAPE; }
+          const long long tiles = gemm_pair_tiles(s, wide);
+          d->shape[4] = wide, d->shape[5] = 1, d->shape[6] = kPairRows, d->shape[7] = 2;
+          set(2 * (int)std::min<long long>(tiles, sm / 2), 1, 1, kUmmaThreads, 1, pair_smem_bytes(wide), 5);
           return BFUSE_OK;
         }
         d->shape[7] = 1;
@@ -850,11 +863,11 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       if ((s[3] * eb) % 16) return shape_err("K rows must be a multiple of 16 bytes (TMA stride rule)");
       if ((s[2] * eb) % 16) return shape_err("N must make output rows a multiple of 16 bytes");
       const bool pairs = act && s[7] == 2;
-      if (act && (s[7] < 0 || s[7] > 2)) return shape_err("shape[7] must be 1 (a CTA per tile) or 2 (pairs of CTAs that walk 256 x 256 tiles)");
-      if (pairs && (bn != kPairTile || bm != kPairTile || split != 1)) return shape_err("shape[7] = 2 (pairs of CTAs) takes 256 x 256 tiles and one k-slice");
-      if (pairs && (kd.gy != 1 || kd.gz != 1 || kd.gx % 2 || kd.gx / 2 > (long long)s[0] * ceil_div(s[1], kPairTile) * ceil_div(s[2], kPairTile)))
-        return shape_err("GridDim of pairs of CTAs must be (2 * pairs, 1, 1), no more pairs than 256 x 256 tiles");
-      if (pairs && k.smem < (size_t)pair_smem_bytes()) return shape_err("shared memory below the ring and the store buffers of a pair");
+      if (act && (s[7] < 0 || s[7] > 2)) return shape_err("shape[7] must be 1 (a CTA per tile) or 2 (pairs of CTAs that walk tiles of 256 rows)");
+      if (pairs && ((bn != 128 && bn != 256) || bm != kPairRows || split != 1)) return shape_err("shape[7] = 2 (pairs of CTAs) takes BM = 256, BN = 128 or 256 and one k-slice");
+      if (pairs && (kd.gy != 1 || kd.gz != 1 || kd.gx % 2 || kd.gx / 2 > gemm_pair_tiles(s, bn)))
+        return shape_err("GridDim of pairs of CTAs must be (2 * pairs, 1, 1), no more pairs than tiles");
+      if (pairs && k.smem < (size_t)pair_smem_bytes(bn)) return shape_err("shared memory below the ring and the store buffers of a pair");
       const int num_kb = ceil_div(s[3] * eb, kUmmaRowBytes), q = ceil_div(num_kb, split);
       if (split > 8 || (split - 1) * q >= num_kb) return shape_err("shape[5] (split) must be 1..8 with every k-slice non-empty");
       if (kd.bx != kUmmaThreads || kd.by != 1 || kd.bz != 1) return shape_err("BlockDim must be (192, 1, 1)");
@@ -876,7 +889,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       std::memset(&p, 0, sizeof(p));
       int rc = encode_map(ctx, &p.map_a, eb, a[0], s[3], s[1], s[0], pairs ? kUmmaBM : bm);
       if (rc) return rc;
-      rc = encode_map(ctx, &p.map_b, eb, a[1], s[3], s[2], s[0], pairs ? kUmmaBM : bn);
+      rc = encode_map(ctx, &p.map_b, eb, a[1], s[3], s[2], s[0], pairs ? bn / 2 : bn);
       if (rc) return rc;
       void *const out = a[act ? 4 : 3];
       rc = encode_map(ctx, &p.map_out, eb, out, s[2], s[1], s[0], 32);
@@ -893,7 +906,7 @@ int build_params(bfuse_context *ctx, KernelRec &k) {
       p.out = out;
       p.batch = s[0], p.M = s[1], p.N = s[2], p.K = s[3];
       p.causal = (int)(d.flags & BFUSE_FLAG_CAUSAL);
-      p.stages = std::min<int>(kUmmaMaxStages, (int)((k.smem - rest) / umma_stage_bytes(bn, bm)));
+      p.stages = pairs ? pair_stages(bn) : std::min<int>(kUmmaMaxStages, (int)((k.smem - rest) / umma_stage_bytes(bn, bm)));
       p.bm = bm;
       p.bn = bn;
       p.split = split;

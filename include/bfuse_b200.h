@@ -65,8 +65,8 @@ enum {
                               /* fp32; accumulated, activated and added in fp32, rounded once; out may not overlap the  */
                               /* inputs otherwise.  BM = 16 or 32 (with                                                 */
                               /* BN = 128 and 1, 2, 4 or 8 k-slices): few rows, multiplied the other way round; the     */
-                              /* runtime's choice for up to 32 rows.  shape[7] = 2 (with BN = BM = 256 and one k-slice): */
-                              /* pairs of CTAs walk 256 x 256 tiles, GridDim (2 * pairs, 1, 1); 1: a CTA per tile; 0:   */
+                              /* runtime's choice for up to 32 rows.  shape[7] = 2 (with BM = 256, BN = 128 or 256 and  */
+                              /* one k-slice): pairs of CTAs walk the tiles, GridDim (2 * pairs, 1, 1); 1: a CTA per tile; 0: */
                               /* pairs for a large product that runs alone (BFUSE_FLAG_SHARE(1)), written back.  A      */
                               /* kernel of pairs is re-tiled for a launch that it shares (bfuse_fusion_info)            */
   BFUSE_OP_RESIDUAL_NORM_BF16 = 10, /* args: x, block, gate|NULL, w|NULL, r|NULL, y|NULL   fparam: eps, scale           */

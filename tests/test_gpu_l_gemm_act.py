@@ -19,6 +19,7 @@ def rt():
 
 
 PAIRS = (256, 1, 256, 2)     # pairs of CTAs that walk 256 x 256 tiles
+NARROW = (128, 1, 256, 2)    # 256 x 128
 
 
 def build(rt, batch, m, n, k, act, bias, other, tiling=(0, 0, 0), seed=0, share=1, std=1.0, grid=None):
@@ -84,7 +85,16 @@ def test_pairs_of_ctas(rt, m, n, k, other):
     run(rt, 2, m, n, k, bf.ACT_NONE, False, other, tiling=PAIRS, grid=(2, 1, 1))      # one pair takes all tiles
 
 
+@pytest.mark.parametrize("m,n,k", [(256, 128, 64), (1, 8, 8), (300, 520, 72), (513, 264, 1096), (129, 2000, 320)])
+@pytest.mark.parametrize("other", [None, "add", "mul"])
+def test_pairs_with_narrow_tiles(rt, m, n, k, other):
+    run(rt, 2, m, n, k, bf.ACT_GELU_TANH, True, other, tiling=NARROW)
+    run(rt, 2, m, n, k, bf.ACT_NONE, False, other, tiling=NARROW, grid=(2, 1, 1))     # one pair takes all tiles
+
+
 def test_pairs_take_several_tiles(rt):
+    run(rt, 1, 2100, 2600, 712, bf.ACT_SILU, True, "mul", tiling=NARROW, grid=(26, 1, 1))   # 189 tiles
+    run(rt, 1, 1500, 4096, 520, bf.ACT_NONE, True, "add")                              # the runtime's choice: narrow
     run(rt, 1, 2100, 2600, 712, bf.ACT_GELU, True, "add", tiling=PAIRS)               # 99 tiles
     run(rt, 1, 2100, 2600, 712, bf.ACT_GELU, True, "add", tiling=PAIRS, grid=(26, 1, 1))
     run(rt, 1, 2048, 4096, 1024, bf.ACT_SILU, False, "mul")                            # the runtime's choice

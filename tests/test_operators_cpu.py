@@ -36,6 +36,11 @@ def test_gemm_act_tilings():
     assert rc == 0 and d.shape[6] == 128
     rc, d = launch(bf.OP_GEMM_ACT_BF16, (1, 4096, 14336, 4096), share=1)      # large and alone: pairs of CTAs
     assert rc == 0 and tuple(d.shape[4:8]) == (256, 1, 256, 2) and d.GridDim.tuple() == (148, 1, 1)
+    rc, d = launch(bf.OP_GEMM_ACT_BF16, (1, 512, 4096, 4096), share=1)        # few tiles: narrow ones
+    assert rc == 0 and tuple(d.shape[4:8]) == (128, 1, 256, 2) and d.GridDim.tuple() == (128, 1, 1)
+    rc, d = launch(bf.OP_GEMM_ACT_BF16, (1, 300, 6000, 2048), share=1)        # a CTA per tile fits the SMs better
+    assert rc == 0 and tuple(d.shape[4:8]) == (128, 1, 128, 1)
+    assert launch(bf.OP_GEMM_ACT_BF16, (1, 512, 4096, 4096, 64, 1, 256, 2), share=1)[0] == 2
     rc, d = launch(bf.OP_GEMM_ACT_BF16, (1, 4096, 14336, 4096), share=2)      # sharing its launch: a CTA per tile, as GEMM_BF16
     _, g = launch(bf.OP_GEMM_BF16, (1, 4096, 14336, 4096), share=2)
     assert rc == 0 and d.shape[7] == 1 and d.GridDim.tuple() == g.GridDim.tuple() and d.smem_bytes == g.smem_bytes
