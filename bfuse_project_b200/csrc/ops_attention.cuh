@@ -14,8 +14,8 @@
 // one sequence times the G query heads of the group, so a single token of a grouped model fills G rows
 // and a prompt's tile reads each key once for the whole group.  BlockDim = (192, 1, 1): warps 0-3 own
 // the rows (thread = row = lane of tensor memory), warp 4 issues the TMA loads, warp 5 the MMAs.  (Eight
-// warps, two threads a row, are no faster: MUFU sets the pace of the exponentials either way, and the two
-// have to exchange their maxima in every block.)
+// warps, two threads a row, are no faster: the two have to exchange their maxima in every block.  Nor are
+// polynomials for an eighth to a half of the exponentials: what MUFU saves, their instructions cost.)
 // GridDim = (slices * kv heads, tiles); the tiles are counted from the sequence offsets on the device
 // (`find_tile`), the host knows only their number at most: (total_q + seqs (P - 1)) / P.  The last
 // tile of a sequence, the one with the most keys under a causal mask, comes first.
@@ -29,6 +29,13 @@
 // there.  It is multiplied the other way round: S^T = K Q^T and O^T += V^T p^T, keys (then dims) in the
 // lanes and the rows in 16 columns; a thread owns a key, p^T goes through shared memory, and S of the next
 // block is made while this one's exponentials are taken.
+//
+// Many short tiles: a CTA that is through its tile takes that of a block that has not started (clusterlaunchcontrol), whose keys
+// are loaded meanwhile; barriers and tensor memory stay.  A block of its own costs 7 us a tile of one block of keys, 3.6 of
+// them beside another CTA's; a walk's tile 2.9.
+//
+// What bounds it: long prompts the softmax between the MMAs of two tiles (a pair of blocks of 128 dims takes 3600 clocks, 2048 of
+// MMAs and 2048 of exponentials) and the power the device may draw; single tokens the loads of the CTA with the longest run of keys.
 //
 // Tensor memory: S in columns 0-127, O in columns 128 up, the bf16 p in 64 columns of its own behind O where
 // there is room (heads of up to 64 in 256 columns; 512 columns where only one CTA fits an SM anyway), else over S.
@@ -54,6 +61,7 @@ enum AttnStatus : int {
   ATTN_WAIT_PROBS_TIMEOUT = 0x305,
   ATTN_WAIT_OUT_TIMEOUT = 0x306,
   ATTN_WAIT_PEERS_TIMEOUT = 0x307,
+  ATTN_WAIT_TILE_TIMEOUT = 0x308,
   ATTN_BAD_OFFSETS = -1,   // BFUSE_STATUS_BAD_OFFSETS: sequence offsets that fall, or that leave the tensors: that sequence is left out
 };
 
@@ -125,15 +133,38 @@ __device__ __forceinline__ float2 ld_shared_f2(uint32_t addr) {
 
 // One tile of queries, as find_tile leaves it in shared memory.
 struct AttnTile {
-  int found;      // 0: this block has no tile
+  int found;      // 0: this block has no tile, -1: a walk ends here
+  int head;       // kv head
   int q0, npos;   // first token, positions (<= P) of the tile
   int kv0, kv_len;
   int last0;      // causal: key index (within the sequence) that the tile's first position may see last
   int keys;       // keys that any row of the tile may see
+  // what came before it in a walk, which says the phase a barrier is in: loads of the ring and of queries; blocks of keys, by tile
+  // of the CTA (one tile: whole tiles, and tiles of few rows); tiles with keys
+  uint32_t loads, queries, blocks[2], outs[2];
 };
 
+// ---- a walk: the CTA asks for the number of a block that has not started, which then never starts ----
+__device__ __forceinline__ void ask_block(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// -1: every block has started
+__device__ __forceinline__ int answered_block(uint32_t answer) {
+  int block;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\tld.shared.b128 a, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tmov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=r"(block)
+      : "r"(answer)
+      : "memory");
+  return block;
+}
+
 // T tiles of one sequence and kv head per CTA: 1, or 2 that share every block of keys (four more warps; whole tiles only).
-template <int T>
+// WALK: a CTA that is through its tile goes on with that of a block that has not started yet, whose keys are loaded meanwhile
+// (alone in its launch, one key slice).
+template <int T, bool WALK>
 struct Attention {
   using Params = AttentionParams;
   static constexpr int kMaxThreads = attn_threads(T);
@@ -145,12 +176,14 @@ struct Attention {
   // The window: [0, 1024) barriers, tensor-memory pointer and the tile; [1024, 2048) what the threads of a row exchange;
   // then Q and the ring of `stages` K / V blocks in the order K0 V0 K1 V1 ...
   struct Window {
-    // s_bar, pv_bar, o_bar, c_bar: one per tile, p_bar: two per tile (few rows: two s_bar and p_bar, by the parity of the block)
-    uint32_t full0, empty0, q_bar, s_bar, p_bar, pv_bar, o_bar, c_bar, stats_bar, join_bar;
+    // s_bar, pv_bar, o_bar, c_bar: one per tile, p_bar: two per tile; few rows: two sf_bar and pf_bar, by the parity of the block;
+    // a walk: tile_bar, the next tile is known, done_bar, all are through one (two each, by the tile's parity: whoever is quick may
+    // be a tile ahead of whoever waits), next_bar, the answer is there
+    uint32_t full0, empty0, q_bar, s_bar, p_bar, pv_bar, o_bar, c_bar, stats_bar, join_bar, sf_bar, pf_bar, pvf_bar, tile_bar, done_bar, next_bar, next;
     uint32_t xch, q, ring, few_join;
     int chunks, tile_bytes;
   };
-  static constexpr int kBars = 2 * kAttnMaxStages + 15;
+  static constexpr int kBars = 2 * kAttnMaxStages + 25;
 
   // Tile number t of the batch (T = 2: pair of tiles) into *tile: sequence i has ceil(len_i / (T P)) of them, the last
   // positions first.  One warp.  Up to 32 sequences: one a lane, the longest first where `sort` (more tiles than run at
@@ -160,7 +193,7 @@ struct Attention {
     const int positions = T * p.positions;
     auto bad = [&] { atomicCAS(status, 0, (int)ATTN_BAD_OFFSETS); };
     auto put = [&](int q0, int q_len, int kv0, int kv_end, int qt) {
-      AttnTile r;
+      AttnTile r = *tile;   // (head, and what came before)
       r.found = kv0 >= 0 && kv_end >= kv0 && kv_end <= p.total_kv;
       if (!r.found) bad();
       r.q0 = q0 + qt * positions;
@@ -237,11 +270,27 @@ struct Attention {
     }
   }
 
-  // of the barriers from q_bar on, those that the 128 threads of a tile arrive at: p_bar (four) and c_bar (two)
-  __device__ __forceinline__ static bool by_threads(const Window &w, int i) {
-    const uint32_t bar = w.q_bar + 8 * i;
-    return (bar >= w.p_bar && bar < w.pv_bar) || (bar >= w.c_bar && bar < w.stats_bar);
+  __device__ __forceinline__ static Window window(const Params &p, uint32_t base) {
+    Window w;
+    w.full0 = base, w.empty0 = w.full0 + 8 * kAttnMaxStages, w.q_bar = w.empty0 + 8 * kAttnMaxStages;
+    w.s_bar = w.q_bar + 8, w.p_bar = w.q_bar + 24, w.pv_bar = w.q_bar + 56, w.o_bar = w.q_bar + 72, w.c_bar = w.q_bar + 88, w.stats_bar = w.q_bar + 104, w.join_bar = w.q_bar + 112;
+    w.sf_bar = w.q_bar + 120, w.pf_bar = w.q_bar + 136, w.pvf_bar = w.q_bar + 152, w.tile_bar = w.q_bar + 160, w.done_bar = w.q_bar + 176, w.next_bar = w.q_bar + 192;
+    w.next = w.full0 + 768, w.xch = w.full0 + 1024, w.q = w.full0 + kUmmaHeaderBytes;
+    w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes, w.few_join = w.ring + p.stages * w.tile_bytes;
+    return w;
   }
+
+  // arrivals at barrier i from q_bar on: the 128 threads of a tile at p_bar (four), c_bar and pf_bar (two each), those of every
+  // tile and the issuer at done_bar
+  __device__ __forceinline__ static int arrivals(const Window &w, int i) {
+    const uint32_t bar = w.q_bar + 8 * i;
+    if (bar == w.done_bar || bar == w.done_bar + 8) return 128 * T + 1;
+    return (bar >= w.p_bar && bar < w.pv_bar) || (bar >= w.c_bar && bar < w.stats_bar) || (bar >= w.pf_bar && bar < w.pvf_bar) ? 128 : 1;
+  }
+  // what came before a tile
+  __device__ __forceinline__ static uint32_t loads(const AttnTile &t) { return WALK ? t.loads : 0u; }
+  __device__ __forceinline__ static uint32_t blocks(const AttnTile &t, int x) { return WALK ? t.blocks[x] : 0u; }
+  __device__ __forceinline__ static uint32_t outs(const AttnTile &t, int x) { return WALK ? t.outs[x] : 0u; }
 
   // this slice's blocks of keys: first and count
   __device__ __forceinline__ static void my_blocks(const AttnTile &t, int split, int slice, int &b0, int &n) {
@@ -263,12 +312,12 @@ struct Attention {
   __device__ __forceinline__ static int sub_blocks(const AttnTile &s, int n) { return T == 1 ? n : (s.keys + kAttnKeys - 1) / kAttnKeys; }
 
   // load i of the ring: K or V of block i / 2
-  __device__ __forceinline__ static void load(const Params &p, const Window &w, const AttnTile &t, int head, int b0, int i, uint32_t slot) {
+  __device__ __forceinline__ static void load(const Params &p, const Window &w, const AttnTile &t, int b0, int i, uint32_t slot) {
     const uint32_t bar = w.full0 + 8 * slot, dst = w.ring + slot * w.tile_bytes;
     const int token = t.kv0 + (b0 + (i >> 1)) * kAttnKeys;
     const CUtensorMap *map = i & 1 ? &p.map_v : &p.map_k;
     mbar_expect_tx(bar, (uint32_t)w.tile_bytes);
-    for (int ch = 0; ch < w.chunks; ++ch) tma_load_3d(dst + ch * kAttnChunkBytes, map, bar, ch * 64, head, token);
+    for (int ch = 0; ch < w.chunks; ++ch) tma_load_3d(dst + ch * kAttnChunkBytes, map, bar, ch * 64, t.head, token);
   }
 
   // 16 finished columns of a row
@@ -285,17 +334,125 @@ struct Attention {
     return p.out + ((size_t)(t.q0 + pos) * p.heads + head * p.group + (row - pos * p.group)) * p.dim;
   }
 
+  __device__ __forceinline__ static void load_q(const Params &p, const Window &w, const AttnTile &t) {
+    const int tiles = T == 2 && t.npos > p.positions ? 2 : 1;
+    mbar_expect_tx(w.q_bar, (uint32_t)(tiles * w.chunks * p.group * p.positions * 128));
+    for (int x = 0; x < tiles; ++x)
+      for (int ch = 0; ch < w.chunks; ++ch)
+        tma_load_3d(w.q + x * w.tile_bytes + ch * kAttnChunkBytes, &p.map_q, w.q_bar, ch * 64, t.head * p.group, t.q0 + x * p.positions);
+  }
+  // loads [from, to) of a tile, each once its slot of the ring is free
+  __device__ __forceinline__ static bool load_run(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int b0, int from, int to) {
+    const uint32_t stages = (uint32_t)p.stages, at = loads(t) + (uint32_t)from;
+    uint32_t s = at % stages, round = at / stages;
+    for (int i = from; i < to; ++i) {
+      if (round > 0 && !mbar_wait(w.empty0 + 8 * s, (round - 1) & 1, c.status, ATTN_WAIT_SLOT_TIMEOUT)) return false;
+      load(p, w, t, b0, i, s);
+      if (++s == stages) s = 0, ++round;
+    }
+    return true;
+  }
+
+  // The loading warp of a walk.  With a tile's last load on its way it asks for the next tile, finds it and loads what the ring has
+  // room for of its keys; the queries wait until everyone is through the tile before.
+  __device__ __forceinline__ static void lead(const Params &p, const TileCtx &c, const Window &w, AttnTile *tile_slot, int loaded, int lane) {
+    AttnTile t = tile_slot[0];
+    bool ok = true;
+    for (int i = 0;; ++i) {
+      int b0 = 0, n = 0;
+      if (t.found) my_blocks(t, 1, 0, b0, n);
+      if (elect_one()) {
+        ok = load_run(p, c, w, t, b0, loaded, 2 * n);
+        mbar_expect_tx(w.next_bar, 16);
+        ask_block(w.next, w.next_bar);
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(w.next_bar, i & 1, c.status, ATTN_WAIT_TILE_TIMEOUT) && ok;
+      const int block = ok ? answered_block(w.next) : -1;
+      fence_async_smem();   // (it has been read: the next one may be written)
+      AttnTile *slot = tile_slot + ((i + 1) & 1);   // everyone is through tile i - 1
+      if (lane == 0) {
+        t.loads += 2 * n;
+        t.queries += n > 0;
+        for (int x = 0; x < 2; ++x) {
+          const int nx = T == 2 ? (n > 0 ? sub_blocks(sub_tile(p, t, x), n) : 0) : few_rows(p, t) == (x == 1) ? n : 0;
+          t.blocks[x] += nx;
+          t.outs[x] += T == 2 ? nx > 0 : n > 0;
+        }
+        t.head = block < 0 ? 0 : block % c.gx;
+        t.found = block < 0 ? -1 : 0;
+        *slot = t;
+      }
+      __syncwarp();
+      if (block >= 0) find_tile(p, block / c.gx, c.gy, lane, slot, c.status);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(w.tile_bar + 8 * ((i + 1) & 1));
+      if (block < 0) return;
+      t = *slot;
+      n = 0;
+      if (t.found) my_blocks(t, 1, 0, b0, n);
+      loaded = min(p.stages, 2 * n);
+      if (elect_one()) {
+        ok = load_run(p, c, w, t, b0, 0, loaded);
+        ok = mbar_wait(w.done_bar + 8 * (i & 1), (i >> 1) & 1, c.status, ATTN_WAIT_TILE_TIMEOUT) && ok;
+        if (ok && n > 0) load_q(p, w, t);
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, ok);
+    }
+  }
+
+  // The issuing warp's part of a tile
+  __device__ __forceinline__ static void issue(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int b0, int n, bool few, uint32_t tmem) {
+    const int stages = p.stages;
+    if (n > 0 && elect_one()) {
+      bool ok = mbar_wait(w.q_bar, WALK ? t.queries & 1 : 0, c.status, ATTN_WAIT_Q_TIMEOUT);
+      if (ok) ok = few ? multiply_few(p, c, w, t, n, tmem) : multiply(p, c, w, t, n, tmem);
+      if (T == 1) umma_commit(w.o_bar);
+      // the releases of the slots' last uses are asynchronous: none may be in flight when the barriers go
+      for (int i = max(0, 2 * n - stages); i < 2 * n && ok; ++i) {
+        const uint32_t at = loads(t) + (uint32_t)i;
+        ok = mbar_wait(w.empty0 + 8 * (at % (uint32_t)stages), (at / (uint32_t)stages) & 1, c.status, ATTN_WAIT_SLOT_TIMEOUT);
+      }
+      for (int x = 0; x < T && ok; ++x) {
+        const int nx = sub_blocks(sub_tile(p, t, x), n);
+        if (nx > 0 && few) ok = mbar_wait(w.pvf_bar, (blocks(t, 1) + nx - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+        if (nx > 0 && !few && p.p_col) ok = mbar_wait(w.pv_bar + 8 * x, (blocks(t, x) + nx - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+        if (nx > 0 && ok) ok = mbar_wait(w.o_bar + 8 * x, outs(t, x) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+      }
+    }
+    __syncwarp();
+  }
+  // The other warps' part (with key slices, where all of them meet the cluster's, every warp's)
+  __device__ __forceinline__ static void rows(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int split, int slice, int b0, int n, bool few, uint32_t tmem) {
+    const int warp = c.tid >> 5;
+    if constexpr (T == 2) {
+      const AttnTile s = sub_tile(p, t, warp >> 2);
+      tile(p, c, w, s, t.head, 1, 0, 0, sub_blocks(s, n), tmem, warp >> 2);
+    } else if (few) {
+      if (t.npos * p.group <= 8) few_tile<8>(p, c, w, t, t.head, split, slice, b0, n, tmem);
+      else few_tile<16>(p, c, w, t, t.head, split, slice, b0, n, tmem);
+    } else {
+      tile(p, c, w, t, t.head, split, slice, b0, n, tmem, 0);
+    }
+  }
+  // tile i of a walk, -1: there is none
+  __device__ __forceinline__ static AttnTile tile_at(const TileCtx &c, const Window &w, const AttnTile *tile_slot, int i) {
+    AttnTile t;
+    t.found = -1;
+    // (tile 0 was there before c.sync)
+    if (i == 0 || warp_wait(w.tile_bar + 8 * (i & 1), ((i - 1) >> 1) & 1, c.status, ATTN_WAIT_TILE_TIMEOUT)) t = tile_slot[i & 1];
+    return t;
+  }
+
   __device__ __forceinline__ static void run(const Params &p, const TileCtx &c) {
     const int warp = c.tid >> 5, lane = c.tid & 31;
-    const int split = p.split, stages = p.stages;
-    const int bx = c.block_x(), slice = bx & (split - 1), head = bx >> log2_of(split);   // (split: a power of two)
-    Window w;
-    w.full0 = smem_u32(c.smem), w.empty0 = w.full0 + 8 * kAttnMaxStages, w.q_bar = w.empty0 + 8 * kAttnMaxStages;
-    w.s_bar = w.q_bar + 8, w.p_bar = w.q_bar + 24, w.pv_bar = w.q_bar + 56, w.o_bar = w.q_bar + 72, w.c_bar = w.q_bar + 88, w.stats_bar = w.q_bar + 104, w.join_bar = w.q_bar + 112;
-    w.xch = w.full0 + 1024, w.q = w.full0 + kUmmaHeaderBytes;
-    w.chunks = attn_chunks(p.dim), w.tile_bytes = w.chunks * kAttnChunkBytes, w.ring = w.q + T * w.tile_bytes, w.few_join = w.ring + stages * w.tile_bytes;
+    const int split = WALK ? 1 : p.split, stages = p.stages;
+    const int slice = c.block_x() & (split - 1);   // (split: a power of two)
+    const Window w = window(p, smem_u32(c.smem));
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(c.smem + 8 * kBars);
-    AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 512);
+    AttnTile *tile_slot = reinterpret_cast<AttnTile *>(c.smem + 512);   // (two, in a walk)
 
     if (warp == kIssuer && !c.tmem_given) {
       tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
@@ -308,10 +465,15 @@ struct Attention {
         mbar_init(w.full0 + 8 * lane, 1);
         mbar_init(w.empty0 + 8 * lane, 1);
       }
-      static_assert(kBars - 2 * kAttnMaxStages <= 32 && 8 * kBars + 4 <= 512, "one lane a barrier, and the header's room");
-      if (lane < kBars - 2 * kAttnMaxStages) mbar_init(w.q_bar + 8 * lane, by_threads(w, lane) ? 128 : 1);
+      static_assert(kBars - 2 * kAttnMaxStages <= 32 && 8 * kBars + 4 <= 512 && 2 * sizeof(AttnTile) <= 256, "one lane a barrier, and the header's room");
+      if (lane < kBars - 2 * kAttnMaxStages) mbar_init(w.q_bar + 8 * lane, arrivals(w, lane));
       if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &p.map_q : lane == 1 ? &p.map_k : &p.map_v) : "memory");
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      if (lane == 0) {
+        tile_slot->head = c.block_x() >> log2_of(split);
+        tile_slot->loads = tile_slot->queries = 0;
+        for (int x = 0; x < 2; ++x) tile_slot->blocks[x] = tile_slot->outs[x] = 0;
+      }
       c.dependency_wait();
       find_tile(p, c.block_y(), c.gy, lane, tile_slot, c.status);
       const AttnTile t = *tile_slot;
@@ -334,12 +496,8 @@ struct Attention {
           }
         }
         if (n > 0) {   // the first round of the ring: every slot is free
-          const int tiles = T == 2 && t.npos > p.positions ? 2 : 1;
-          mbar_expect_tx(w.q_bar, (uint32_t)(tiles * w.chunks * p.group * p.positions * 128));
-          for (int x = 0; x < tiles; ++x)
-            for (int ch = 0; ch < w.chunks; ++ch)
-              tma_load_3d(w.q + x * w.tile_bytes + ch * kAttnChunkBytes, &p.map_q, w.q_bar, ch * 64, head * p.group, t.q0 + x * p.positions);
-          for (int i = 0; i < loaded; ++i) load(p, w, t, head, b0, i, (uint32_t)i);
+          load_q(p, w, t);
+          for (int i = 0; i < loaded; ++i) load(p, w, t, b0, i, (uint32_t)i);
         }
       }
       __syncwarp();
@@ -352,51 +510,52 @@ struct Attention {
     // this CTA's barriers are up: its peers may push (they wait for that only when they have something to push)
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const uint32_t tmem = c.tmem_given ? c.tmem_base : *reinterpret_cast<volatile uint32_t *>(tmem_slot);
-    const AttnTile t = *tile_slot;
-    if (t.found) {   // (the same for every CTA of a cluster)
-      int b0, n;
-      my_blocks(t, split, slice, b0, n);
-      const bool few = few_rows(p, t);
+    int b0, n;
+    if constexpr (WALK) {
       if (warp == kProducer) {
-        if (n > 0 && elect_one()) {
-          uint32_t s = loaded == stages ? 0 : (uint32_t)loaded, ph = 0;
-          for (int i = loaded; i < 2 * n; ++i) {
-            if (!mbar_wait(w.empty0 + 8 * s, ph, c.status, ATTN_WAIT_SLOT_TIMEOUT)) break;
-            load(p, w, t, head, b0, i, s);
-            if (++s == (uint32_t)stages) s = 0, ph ^= 1;
-          }
-        }
-        __syncwarp();
+        lead(p, c, w, tile_slot, loaded, lane);
       } else if (warp == kIssuer) {
-        if (n > 0 && elect_one()) {
-          bool ok = mbar_wait(w.q_bar, 0, c.status, ATTN_WAIT_Q_TIMEOUT);
-          if (ok) ok = few ? multiply_few(p, c, w, n, tmem) : multiply(p, c, w, t, n, tmem);
-          if (T == 1) umma_commit(w.o_bar);
-          // the releases of the slots' last uses are asynchronous: none may be in flight when the barriers go
-          for (int i = max(0, 2 * n - stages); i < 2 * n && ok; ++i)
-            ok = mbar_wait(w.empty0 + 8 * (i % stages), (i / stages) & 1, c.status, ATTN_WAIT_SLOT_TIMEOUT);
-          for (int x = 0; x < T && ok; ++x) {
-            const int nx = sub_blocks(sub_tile(p, t, x), n);
-            if (nx > 0 && (few || p.p_col)) ok = mbar_wait(w.pv_bar + 8 * x, (nx - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
-            if (nx > 0 && ok) ok = mbar_wait(w.o_bar + 8 * x, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+#pragma unroll 1
+        for (int i = 0;; ++i) {
+          const AttnTile t = tile_at(c, w, tile_slot, i);
+          if (t.found < 0) break;
+          if (t.found) {
+            my_blocks(t, 1, 0, b0, n);
+            issue(p, c, w, t, b0, n, few_rows(p, t), tmem);
           }
+          if (elect_one()) mbar_arrive(w.done_bar + 8 * (i & 1));
+          __syncwarp();
         }
-        __syncwarp();
-      }
-      if constexpr (T == 2) {
-        const int x = warp >> 2;   // (the loading and issuing warps: 2, no tile)
-        if (x < T) {
-          const AttnTile s = sub_tile(p, t, x);
-          tile(p, c, w, s, head, 1, 0, 0, sub_blocks(s, n), tmem, x);
-        }
-      } else if (few) {
-        if (t.npos * p.group <= 8) few_tile<8>(p, c, w, t, head, split, slice, b0, n, tmem);
-        else few_tile<16>(p, c, w, t, head, split, slice, b0, n, tmem);
       } else {
-        tile(p, c, w, t, head, split, slice, b0, n, tmem, 0);
+#pragma unroll 1
+        for (int i = 0;; ++i) {
+          const AttnTile t = tile_at(c, w, tile_slot, i);
+          if (t.found < 0) break;
+          if (t.found) {
+            my_blocks(t, 1, 0, b0, n);
+            rows(p, c, window(p, anew(w.full0)), t, 1, 0, b0, n, few_rows(p, t), anew(tmem));
+          }
+          __syncwarp();
+          fence_async_smem();   // what this thread wrote over the queries comes before the next ones
+          tc_fence_before();
+          mbar_arrive(w.done_bar + 8 * (i & 1));
+        }
       }
-    } else if (split > 1) {
-      cluster_wait();
+    } else {
+      const AttnTile t = *tile_slot;
+      if (t.found) {   // (the same for every CTA of a cluster)
+        my_blocks(t, split, slice, b0, n);
+        const bool few = few_rows(p, t);
+        if (warp == kProducer) {
+          if (n > 0 && elect_one()) load_run(p, c, w, t, b0, loaded, 2 * n);
+          __syncwarp();
+        } else if (warp == kIssuer) {
+          issue(p, c, w, t, b0, n, few, tmem);
+        }
+        rows(p, c, w, t, split, slice, b0, n, few, tmem);
+      } else if (split > 1) {
+        cluster_wait();
+      }
     }
     __syncwarp();
     tc_fence_before();
@@ -415,6 +574,14 @@ struct Attention {
 
   __device__ __forceinline__ static void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+  // In a walk the compiler would compute all that follows from x once, before the first tile, and hold it in registers that a row's
+  // scores need (396 bytes of spills, prompts a fifth slower): x is another one for every tile.
+  template <class V>
+  __device__ __forceinline__ static V anew(V x) {
+    if (WALK) asm volatile("" : "+r"(x));
+    return x;
+  }
+
   // ---- whole tiles: rows in the lanes ----
 
   // A slot of the ring and the phase its barrier is in, carried along: loads are `step` apart (divisions would idle the tensor pipe).
@@ -425,6 +592,9 @@ struct Attention {
       if (slot >= stages) slot -= stages, phase ^= 1;
     }
   };
+  __device__ __forceinline__ static RingAt ring_at(const AttnTile &t, uint32_t load, uint32_t stages) {   // load 0 or 1 of the tile
+    return WALK ? RingAt{(t.loads + load) % stages, (t.loads + load) / stages & 1u} : RingAt{load, 0};
+  }
 
   // S = Q K^T of tile x and the block of keys at k; `wait`: nobody has waited for them yet, `last`: no other tile reads them after it
   __device__ __forceinline__ static bool scores(const Params &p, const TileCtx &c, const Window &w, const RingAt &k, uint32_t tmem, int x, bool wait, bool last) {
@@ -453,7 +623,8 @@ struct Attention {
     const uint32_t idesc = umma_idesc(1, w.chunks * 64) | (1u << 16), stages = (uint32_t)p.stages;
     int nx[2] = {n, 0};
     if (T == 2) nx[0] = sub_blocks(sub_tile(p, t, 0), n), nx[1] = sub_blocks(sub_tile(p, t, 1), n);
-    RingAt k{0, 0}, v{1, 0};
+    RingAt k = ring_at(t, 0, stages), v = ring_at(t, 1, stages);
+    const uint32_t g[2] = {blocks(t, 0), T == 2 ? blocks(t, 1) : 0u};
     // block j is read by tile 0, if that has so many, and then by tile 1: the first waits for it, the last gives it up
     auto first = [&](int j, int x) { return T == 1 || x == 0 || j >= nx[0]; };
     auto last = [&](int j, int x) { return T == 1 || x == 1 || j >= nx[1]; };
@@ -467,7 +638,7 @@ struct Attention {
         if (T == 2 && j >= nx[x]) continue;
         const bool more = j + 1 < nx[x];
         if (p.p_col && more) {
-          if (!mbar_wait(w.c_bar + 8 * x, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
+          if (!mbar_wait(w.c_bar + 8 * x, (g[x] + j) & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
           tc_fence_after();
           if (!scores(p, c, w, k, tmem, x, first(j + 1, x), last(j + 1, x))) return false;
         }
@@ -475,7 +646,7 @@ struct Attention {
         const uint32_t pt = tmem + 256u * x + (uint32_t)p.p_col;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(w.p_bar + 16 * x + 8 * half, j & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
+          if (!mbar_wait(w.p_bar + 16 * x + 8 * half, (g[x] + j) & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT)) return false;
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -501,9 +672,9 @@ struct Attention {
 
   // Values past the end of the sequence are the next one's, or whatever the buffer holds: p is 0 there, but 0 * NaN is not,
   // so those rows of V become zeros.  `first` of `threads` threads; the block's V is load 2 j + 1 of the ring.
-  __device__ __forceinline__ static bool clear_tail(const Params &p, const TileCtx &c, const Window &w, int j, int have, int first, int threads) {
-    const int i = 2 * j + 1, s = i % p.stages;
-    const bool ok = warp_wait(w.full0 + 8 * s, (i / p.stages) & 1, c.status, ATTN_WAIT_KV_TIMEOUT);
+  __device__ __forceinline__ static bool clear_tail(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int j, int have, int first, int threads) {
+    const uint32_t i = loads(t) + 2u * j + 1u, s = i % (uint32_t)p.stages;
+    const bool ok = warp_wait(w.full0 + 8 * s, (i / (uint32_t)p.stages) & 1, c.status, ATTN_WAIT_KV_TIMEOUT);
     const uint32_t v = w.ring + s * w.tile_bytes;
     if (ok)
       for (int ch = 0; ch < w.chunks; ++ch)
@@ -518,12 +689,27 @@ struct Attention {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
   }
-  // The 128 scores of a row: the largest (with m), then 32 of their exponentials as bf16 into tensor memory
-  template <bool MASKED>
-  __device__ __forceinline__ static float largest(uint32_t (&r)[4][32], int seen, float m) {
+  // columns behind `seen` of a row's scores do not count
+  template <int G>
+  __device__ __forceinline__ static void mask(uint32_t (&r)[G][32], int seen) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (32 * g + i > seen) r[g][i] = __float_as_uint(-INFINITY);
+  }
+  // The values of a tcgen05.ld that has been waited for: no use of them may move before the wait
+  __device__ __forceinline__ static void loaded_scores(uint32_t (&r)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+  }
+  // The scores of a row: the largest of G x 32 (with m), then 32 of their exponentials as bf16 into tensor memory
+  template <bool MASKED, int G>
+  __device__ __forceinline__ static float largest(uint32_t (&r)[G][32], int seen, float m) {
     float mx[4] = {m, m, m, m};
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         if (MASKED && 32 * g + i > seen) r[g][i] = __float_as_uint(-INFINITY);
@@ -548,19 +734,20 @@ struct Attention {
   __device__ __forceinline__ static void tile(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice,
                                               int b0, int n, uint32_t tmem_base, int x) {
     const uint32_t tmem = tmem_base + 256u * x;
-    const int warp = c.tid >> 5, lane = c.tid & 31;
-    const int quad = (threadIdx.x >> 5) & 3;   // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
+    const int tid = anew(c.tid), warp = tid >> 5, lane = tid & 31;
+    const int quad = (anew(threadIdx.x) >> 5) & 3;   // hardware warp w may only touch TMEM lanes [32 * (w % 4), +32)
     const int rows = t.npos * p.group, row = quad * 32 + lane, active = (rows + 31) >> 5;
     const bool mine = warp < kProducer && quad < active;   // this warp owns rows (the others only keep the barriers going)
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
     float m = -INFINITY, l = 0.f;   // the maximum the exponentials are taken against, and their sum
     bool ok = true;
+    const uint32_t before = blocks(t, x);
     const uint32_t s_bar = w.s_bar + 8 * x, p_bar = w.p_bar + 16 * x, pv_bar = w.pv_bar + 8 * x, c_bar = w.c_bar + 8 * x;
     if (!mine && warp < kProducer) {
       for (int j = 0; j < n && ok; ++j) {
-        ok = warp_wait(s_bar, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        ok = warp_wait(s_bar, (before + j) & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
         if (p.p_col) mbar_arrive(c_bar);
-        if (p.p_col && j > 0 && ok) ok = warp_wait(pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+        if (p.p_col && j > 0 && ok) ok = warp_wait(pv_bar, (before + j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
         mbar_arrive(p_bar);
         mbar_arrive(p_bar + 8);
       }
@@ -571,21 +758,32 @@ struct Attention {
 #pragma unroll 1
       for (int j = 0; j < n && ok; ++j) {
         const int key0 = (b0 + j) * kAttnKeys;
-        ok = warp_wait(s_bar, j & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
+        ok = warp_wait(s_bar, (before + j) & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[4][32];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) tmem_ld_32x32(trow + 32 * g, r[g]);
-        tmem_ld_wait();
-        if (p.p_col) {
-          tc_fence_before();
-          mbar_arrive(c_bar);   // S may be overwritten
-        }
         const int seen = limit - key0;   // columns 0..seen of this block count
-        const float mx = __any_sync(0xffffffffu, seen < kAttnKeys - 1) ? largest<true>(r, seen, m) : largest<false>(r, seen, m);
+        const bool masked = __any_sync(0xffffffffu, seen < kAttnKeys - 1);
+        // A row's 128 scores at once; in a walk, which leaves fewer registers, the second 64 twice, for the maximum and for their
+        // exponentials (with all at once 276 bytes of spills: 60 prompts of 256 tokens 49 us, so 44; without a walk 57 and 58).
+        constexpr int G = WALK ? 2 : 4;
+        uint32_t r[G][32];
+        float mx = m;
+#pragma unroll
+        for (int col = kAttnKeys - 32 * G; col >= 0; col -= 32 * G) {
+#pragma unroll
+          for (int g = 0; g < G; ++g) tmem_ld_32x32(trow + col + 32 * g, r[g]);
+          tmem_ld_wait();
+          if (!WALK && p.p_col) {
+            tc_fence_before();
+            mbar_arrive(c_bar);   // S may be overwritten
+          }
+          if (WALK)
+#pragma unroll
+            for (int g = 0; g < G; ++g) loaded_scores(r[g]);
+          mx = masked ? largest<true>(r, seen - col, mx) : largest<false>(r, seen - col, mx);
+        }
         if (p.p_col && j > 0) {   // p's columns are free, and O is whole, once p V of block j - 1 is done
-          ok = warp_wait(pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          ok = warp_wait(pv_bar, (before + j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
           tc_fence_after();
         }
         // O follows a larger maximum only when that grew by more than 2^8: p stays below 2^8 and the sums in fp32 lose
@@ -607,24 +805,34 @@ struct Attention {
           }
         }
         const int have = t.kv_len - key0;
-        if (have < kAttnKeys && ok) ok = clear_tail(p, c, w, j, have, row, active * 32);
+        if (have < kAttnKeys && ok) ok = clear_tail(p, c, w, t, j, have, row, active * 32);
         const float mc = m == -INFINITY ? 0.f : m * sc;
-        float2 sum[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) sum[i] = make_float2(0.f, 0.f);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const uint32_t pt = trow + (uint32_t)p.p_col;   // (over S, p of the first 64 keys stays clear of the scores of the others)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          exponentials(trow + (uint32_t)p.p_col + 16 * g, r[g], sc, mc, sum);
+          exponentials(pt + 16 * g, r[g & (G - 1)], sc, mc, sum);
+          if (WALK && g < 2) tmem_ld_32x32(trow + 64 + 32 * g, r[g]);
           if (g & 1) {
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(p_bar + 8 * (g >> 1));
           }
+          if (WALK && g == 1) {
+            tmem_ld_wait();
+            loaded_scores(r[0]);
+            loaded_scores(r[1]);
+            if (p.p_col) {
+              tc_fence_before();
+              mbar_arrive(c_bar);   // S may be overwritten
+            }
+            if (masked) mask(r, seen - 64);
+          }
         }
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
-      if (ok) ok = warp_wait(w.o_bar + 8 * x, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+      if (ok) ok = warp_wait(w.o_bar + 8 * x, outs(t, x) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
       tc_fence_after();
     }
     if (T == 1 && split > 1) {
@@ -726,16 +934,17 @@ struct Attention {
 
   // p^T of a block: 16 rows x 128 keys bf16, K-major in two 64-key chunks; two of them lie over the rows of the Q tile that a
   // tile of few rows does not have
-  __device__ __forceinline__ static uint32_t pt_smem(const Window &w, int j) { return w.q + 2048u + (uint32_t)(j & 1) * 4096u; }
+  __device__ __forceinline__ static uint32_t pt_smem(const Window &w, uint32_t j) { return w.q + 2048u + (j & 1) * 4096u; }
 
   // S^T of block j + 1 = K Q^T goes into the other of two buffers while the threads work on block j (block j - 1 is done with
   // it), then O^T += V^T p^T of block j.  The ring's loads are used in the order K0 K1 V0 K2 V1 ...
-  __device__ __forceinline__ static bool multiply_few(const Params &p, const TileCtx &c, const Window &w, int n, uint32_t tmem) {
+  __device__ __forceinline__ static bool multiply_few(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int n, uint32_t tmem) {
     const uint32_t idesc_s = umma_idesc(1, kAttnFewRows), idesc_o = idesc_s | (1u << 15), stages = (uint32_t)p.stages;   // V transposed
     const uint32_t q_lo = k_major_desc(w.q), chunk_step = w.chunks == 2 ? kAttnChunkBytes : 0;   // (a head of one chunk fills 64 lanes, the others get it again)
     const int ksteps = (p.dim + 15) >> 4;
-    RingAt k{0, 0}, v{1, 0};
+    RingAt k = ring_at(t, 0, stages), v = ring_at(t, 1, stages);
     for (int j = -1; j < n; ++j) {
+      const uint32_t g = blocks(t, 1) + (uint32_t)j;
       if (j + 1 < n) {
         if (!mbar_wait(w.full0 + 8 * k.slot, k.phase, c.status, ATTN_WAIT_KV_TIMEOUT)) return false;
         tc_fence_after();
@@ -743,24 +952,24 @@ struct Attention {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t off = (uint32_t)(i >> 2) * (kAttnChunkBytes >> 4) + 2 * (i & 3);
-          if (i < ksteps) umma_ss<1>(tmem + (uint32_t)((j + 1) & 1) * kAttnFewRows, k_lo + off, q_lo + off, idesc_s, i > 0);
+          if (i < ksteps) umma_ss<1>(tmem + ((g + 1) & 1) * kAttnFewRows, k_lo + off, q_lo + off, idesc_s, i > 0);
         }
         umma_commit(w.empty0 + 8 * k.slot);
-        umma_commit(w.s_bar + 8 * ((j + 1) & 1));
+        umma_commit(w.sf_bar + 8 * ((g + 1) & 1));
         k.advance(2, stages);
       }
       if (j < 0) continue;
       // (the next block's p may be there before this wait is: a barrier for each of the two)
       if (!mbar_wait(w.full0 + 8 * v.slot, v.phase, c.status, ATTN_WAIT_KV_TIMEOUT) ||
-          !mbar_wait(w.p_bar + 8 * (j & 1), (j >> 1) & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT))
+          !mbar_wait(w.pf_bar + 8 * (g & 1), (g >> 1) & 1, c.status, ATTN_WAIT_PROBS_TIMEOUT))
         return false;
       tc_fence_after();
-      const uint32_t v_lo = v_desc(w.ring + v.slot * w.tile_bytes, chunk_step), pt_lo = k_major_desc(pt_smem(w, j));
+      const uint32_t v_lo = v_desc(w.ring + v.slot * w.tile_bytes, chunk_step), pt_lo = k_major_desc(pt_smem(w, g));
 #pragma unroll
       for (int i = 0; i < kAttnKeys / 16; ++i)
         umma_ss<1>(tmem + 128, v_lo + 128 * i, pt_lo + (uint32_t)(i >> 2) * 128 + 2 * (i & 3), idesc_o, j > 0 || i > 0);
       umma_commit(w.empty0 + 8 * v.slot);
-      umma_commit(w.pv_bar);
+      umma_commit(w.pvf_bar);
       v.advance(2, stages);
     }
     return true;
@@ -823,7 +1032,7 @@ struct Attention {
   template <int R>   // rows worked on: 8 or 16
   __device__ __forceinline__ static void few_tile(const Params &p, const TileCtx &c, const Window &w, const AttnTile &t, int head, int split, int slice,
                                                   int b0, int n, uint32_t tmem) {
-    const int warp = c.tid >> 5, lane = c.tid & 31, quad = (threadIdx.x >> 5) & 3, at = quad * 32 + lane;   // key of the block, then dim
+    const int tid = anew(c.tid), warp = tid >> 5, lane = tid & 31, quad = (anew(threadIdx.x) >> 5) & 3, at = quad * 32 + lane;   // key of the block, then dim
     const bool mine = warp < 4;
     const int rows = t.npos * p.group;
     const uint32_t tlane = tmem + ((uint32_t)(quad * 32) << 16);
@@ -837,10 +1046,11 @@ struct Attention {
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
         const int key0 = (b0 + j) * kAttnKeys, key = key0 + at;
-        if (ok) ok = warp_wait(w.s_bar + 8 * (j & 1), (j >> 1) & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);   // (these four warps meet in every block: they go on together after a wait that gave up)
+        const uint32_t g = blocks(t, 1) + (uint32_t)j;
+        if (ok) ok = warp_wait(w.sf_bar + 8 * (g & 1), (g >> 1) & 1, c.status, ATTN_WAIT_SCORES_TIMEOUT);   // (these four warps meet in every block: they go on together after a wait that gave up)
         tc_fence_after();
         uint32_t r[R];
-        tmem_ld_rows<R>(tlane + (uint32_t)(j & 1) * kAttnFewRows, r);
+        tmem_ld_rows<R>(tlane + (g & 1) * kAttnFewRows, r);
         float s[R];
         bool grown = false;
 #pragma unroll
@@ -868,7 +1078,7 @@ struct Attention {
             mx[i] = f;
           }
           if (j > 0) {   // block j - 1 has to be in O
-            if (ok) ok = warp_wait(w.pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+            if (ok) ok = warp_wait(w.pvf_bar, (g - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
             tc_fence_after();
             uint32_t o[R];
             tmem_ld_rows<R>(tlane + 128, o);
@@ -878,7 +1088,7 @@ struct Attention {
           }
         }
         // (S of this block stands for block j - 2's products, which read this buffer: it was issued after them)
-        const uint32_t pt = pt_smem(w, j) + (uint32_t)(at >> 6) * 2048u + (uint32_t)(at & 7) * 2u;
+        const uint32_t pt = pt_smem(w, g) + (uint32_t)(at >> 6) * 2048u + (uint32_t)(at & 7) * 2u;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const float e = exp2_approx(s[i] - (m[i] == -INFINITY ? 0.f : m[i]));
@@ -889,14 +1099,14 @@ struct Attention {
         const int have = t.kv_len - key0;
         if (have < kAttnKeys) {
           // (these threads may be a block ahead: V's barrier says which block it holds only once block j - 1 is through)
-          if (j > 0 && ok) ok = warp_wait(w.pv_bar, (j - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
-          if (ok) ok = clear_tail(p, c, w, j, have, at, 128);
+          if (j > 0 && ok) ok = warp_wait(w.pvf_bar, (g - 1) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
+          if (ok) ok = clear_tail(p, c, w, t, j, have, at, 128);
         }
         fence_async_smem();
         tc_fence_before();
-        mbar_arrive(w.p_bar + 8 * (j & 1));
+        mbar_arrive(w.pf_bar + 8 * (g & 1));
       }
-      if (ok) ok = warp_wait(w.o_bar, 0, c.status, ATTN_WAIT_OUT_TIMEOUT);
+      if (ok) ok = warp_wait(w.o_bar, outs(t, 0) & 1, c.status, ATTN_WAIT_OUT_TIMEOUT);
       tc_fence_after();
       quads_reduce<OpSum, R>(c, w, quad, lane, l);
     }
@@ -961,7 +1171,8 @@ struct Attention {
   }
 };
 
-using AttentionBf16 = Attention<1>;
-using AttentionBf16Two = Attention<2>;
+using AttentionBf16 = Attention<1, false>;
+using AttentionBf16Walk = Attention<1, true>;
+using AttentionBf16Two = Attention<2, false>;
 
 }  // namespace bfuse

@@ -68,6 +68,12 @@ struct RowFiller<I, kNumOps> {
   static void fill(PairEntry *) {}
 };
 
+// attention alone in its launch: two tiles per CTA, or a walk
+template <class Two, class Walk>
+cudaError_t launch_alone(const DispatchTable &t, const void *pa, unsigned grid, unsigned block, size_t smem, cudaStream_t s) {
+  return block == (unsigned)Two::kMaxThreads ? launch_single<Two>(t, pa, grid, block, smem, s) : launch_single<Walk>(t, pa, grid, block, smem, s);
+}
+
 template <>
 void fill_pair_row<BFUSE_ROW>(PairEntry *row, SingleEntry *single) {
   using A = typename OpAt<BFUSE_ROW>::type;
@@ -80,7 +86,7 @@ void fill_pair_row<BFUSE_ROW>(PairEntry *row, SingleEntry *single) {
     single->launch = &launch_single<A>;
     single->attr = &attr_single<A>;
     single->launch_other = nullptr;
-    if constexpr (std::is_same<A, AttentionBf16>::value) single->launch_other = &launch_single<AttentionBf16Two>;
+    if constexpr (std::is_same<A, AttentionBf16>::value) single->launch_other = &launch_alone<AttentionBf16Two, AttentionBf16Walk>;
     if constexpr (std::is_same<A, GemmUmma<1, true>>::value) single->launch_other = &launch_single<GemmActPairs>;
   }
   single->group = &launch_group<A>;

@@ -309,6 +309,15 @@ int attention_slices(const int *s, int share, int sm) {
   return 1;
 }
 
+// CTAs that walk (Attention<1, true>): two and a half times as many blocks as run at once, of few rows or of 512 keys on the
+// average (us, without and with: 100 single tokens over up to 1500 keys, 8 kv heads 72 / 66, 500 over up to 64 keys 55 / 41;
+// 100 prompts of 64 tokens, 12 heads 41 / 33, 60 of 256 57 / 44, 64 of 512 141 / 134; 16 of 1024 76 / 92; two rounds of blocks,
+// 16 prompts of up to 512, 22 / 25).
+bool attention_walks(const int *s, int cluster, int grid, size_t smem, int sm) {
+  if (cluster != 1 || s[9] == 2 || grid < (smem > kAttnHalfSm ? 1 : 2) * sm * 5 / 2) return false;
+  return (long long)s[2] <= 512LL * s[0] || (long long)s[1] * (s[3] / s[4]) <= (long long)kAttnFewRows * s[0];
+}
+
 int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *err) {
   const int *s = d->shape;
   auto set = [&](int gx, int gy, int gz, int bx, int by, size_t smem, int nargs) {
@@ -1023,8 +1032,9 @@ bool lone(const KernelRec &k) {
   return k.desc.op == BFUSE_OP_GEMM_ACT_BF16 && k.desc.shape[7] == 2;
 }
 // Is it launched by the second kernel of its operator?
-bool other_kernel(const KernelRec &k) {
-  return whole_planes(k) || (k.desc.op == BFUSE_OP_ATTENTION_BF16 && k.desc.shape[9] == 2) || (k.desc.op == BFUSE_OP_GEMM_ACT_BF16 && k.desc.shape[7] == 2);
+bool other_kernel(const bfuse_context *ctx, const KernelRec &k) {
+  if (k.desc.op == BFUSE_OP_ATTENTION_BF16) return k.desc.shape[9] == 2 || attention_walks(k.desc.shape, k.cluster, k.dims.grid(), k.smem, ctx->sm_count);
+  return whole_planes(k) || (k.desc.op == BFUSE_OP_GEMM_ACT_BF16 && k.desc.shape[7] == 2);
 }
 
 DispatchTable single_table(const bfuse_context *ctx, const KernelRec &k) {
@@ -1060,7 +1070,7 @@ int launch_one(bfuse_context *ctx, KernelRec &k, cudaStream_t s) {
   const DispatchTable t = single_table(ctx, k);
   const size_t smem = k.smem + 1024;
   const SingleEntry &se = ctx->singles[k.desc.op];
-  cudaError_t e = (other_kernel(k) ? se.launch_other : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
+  cudaError_t e = (other_kernel(ctx, k) ? se.launch_other : se.launch)(t, k.params, (unsigned)k.dims.grid(), (unsigned)k.dims.block(), smem, s);
   if (e != cudaSuccess) return fail_cuda(ctx, e, ("launch " + k.name).c_str());
   return BFUSE_OK;
 }

@@ -124,6 +124,23 @@ def test_single_tokens_with_more_tiles_than_fit_at_once(rt):
     run(rt, [2] * 40, [1500] * 40, 32, 4, 64, True)      # 16 rows a tile
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,causal,seqs", [(32, 8, 128, True, 60), (12, 12, 64, False, 40), (12, 12, 64, True, 30), (8, 8, 128, False, 50),
+                                                            (16, 2, 40, True, 300)])
+def test_blocks_take_tile_after_tile(rt, heads, kv_heads, dim, causal, seqs):
+    # more tiles than run at once: of few rows and whole, without queries, without keys, of one block and of several
+    rng = np.random.default_rng(seqs)
+    q_lens = [int(n) for n in rng.choice([0, 1, 1, 2, 31, 128, 200], seqs)]
+    kv_lens = [int(n) for n in rng.choice([0, 1, 90, 128, 129, 400, 700], seqs)]
+    run(rt, q_lens, kv_lens, heads, kv_heads, dim, causal)
+    run(rt, [1] * seqs * 8, [int(n) for n in rng.choice([0, 3, 128, 300], seqs * 8)], heads, kv_heads, dim, causal)
+
+
+def test_pairs_of_tiles_take_pair_after_pair(rt):
+    run(rt, [2100, 4300], [2100, 4300], 16, 16, 64, True)
+    run(rt, [3000, 300], [4096, 300], 12, 12, 128, False)
+    run(rt, [4500, 700], [200, 4200], 16, 16, 128, True)    # most queries without keys
+
+
 def test_large_scores_and_growing_maximum(rt):
     import torch
     # keys whose scores rise along the sequence: the running maximum moves at every block
