@@ -1073,9 +1073,9 @@ struct GemmUmma {
 // BlockDim = (192, 1, 1), warps as in GemmUmma; the MMAs are issued by the cluster's first CTA.  Every CTA loads its own
 // operands and reports them to the first one's barriers; a stage is given up, and an accumulator announced, in both.
 //
-// What bounds them: a K block of a 256 x 256 tile passes through each SM's shared memory as 32 KB written and 48 KB read, 640
-// clocks at 128 bytes a clock, its MMAs take 512 (and large products the power the device may draw).  A tile of 256 x 128
-// takes 56 KB a K block, 437 clocks, for 256 of MMAs: for products of few tiles, which then spread over twice the SMs.
+// What bounds them: the tensor pipe, 81 % busy in the SMs' active clocks (4096 x 14336 x 2048), at the clock that the power limit
+// leaves.  Tiles of 256 x 128 are for products of few tiles, which then spread over twice the SMs: a K block's MMAs are half as
+// long (256 clocks), but it takes 400 clocks of 24 KB of loads, so not where the wide tiles fill the device.
 constexpr int kPairRows = 256, kPairBufs = 3;
 __host__ __device__ constexpr int pair_stages(int bn) { return bn == 256 ? 5 : 7; }
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return kUmmaABytes + bn / 2 * kUmmaRowBytes; }   // 128 rows of A, half of W's

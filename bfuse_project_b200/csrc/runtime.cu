@@ -229,8 +229,7 @@ bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
 long long gemm_pair_tiles(const int *s, int bn) { return (long long)s[0] * ceil_div(s[1], kPairRows) * ceil_div(s[2], bn); }
 // Pairs of CTAs that walk tiles of 256 rows and *bn columns (GemmActPairs): alone in its launch, where the runtime may choose the
 // tiling.  What a K block costs an SM, as measured: 15 in a 256 x 256 tile (0.28 us), 9 in a 256 x 128 one, 10 in a 128 x 128
-// tile of its own -- every operand is written to shared memory and read from there, and that sets the pace -- and the last
-// wide tile's epilogue, which no MMA covers, as much as 8 K blocks.  (us, wide / narrow / a CTA per tile: 512 x 4096 x 4096
+// tile of its own -- the narrower ones wait for their loads, 24 and 32 KB a K block and SM -- and the last wide tile's epilogue, which no MMA covers, as much as 8 K blocks.  (us, wide / narrow / a CTA per tile: 512 x 4096 x 4096
 // 28.5 / 19.4 / 20.6, 1024 x 4096 x 4096 29.9 / 32.1 / 35.7, 1500 x 4096 x 4096 49.0 / 44.5 / 57.7, 2048 x 2048 x 2048 19.4 /
 // 17.9 / 19.5, 300 x 6000 x 2048 23.0 / 21.2 / 14.1.)  Not for fewer tiles than half the pairs: 256 x 4096 x 4096 17.0, 15.5 in
 // tiles of 64 columns.
