@@ -135,6 +135,38 @@ def test_blocks_take_tile_after_tile(rt, heads, kv_heads, dim, causal, seqs):
     run(rt, [1] * seqs * 8, [int(n) for n in rng.choice([0, 3, 128, 300], seqs * 8)], heads, kv_heads, dim, causal)
 
 
+def test_two_launches_take_their_own_tiles(rt):
+    import torch
+    sets = []
+    for seed in (1, 2):
+        lens = [int(n) for n in np.random.default_rng(seed).choice([1, 60, 128, 150], 120)]
+        q, k, v = tensors(torch, lens, lens, 12, 12, 64, seed)
+        out, cu = torch.empty_like(q), cumulative(torch, lens)
+        sets.append((lens, q, k, v, out, cu, kernel(rt, q, k, v, cu, None, out, 0.125, True), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side = torch.cuda.current_stream()
+        for *_, h, stream in sets:
+            stream.wait_stream(side)
+            rt.launch_kernel(h, stream.cuda_stream)
+            rt.launch_kernel(h, stream.cuda_stream)
+            side.wait_stream(stream)
+    for direct in (True, False):
+        for s in sets:
+            s[4].zero_()
+        torch.cuda.synchronize()
+        if direct:
+            for *_, h, stream in sets:
+                rt.launch_kernel(h, stream.cuda_stream)
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert rt.read_status() == 0
+        for lens, q, k, v, out, *_ in sets:
+            check(torch, out, *reference(torch, q, k, v, lens, lens, 0.125, True))
+
+
 def test_pairs_of_tiles_take_pair_after_pair(rt):
     run(rt, [2100, 4300], [2100, 4300], 16, 16, 64, True)
     run(rt, [3000, 300], [4096, 300], 12, 12, 128, False)
