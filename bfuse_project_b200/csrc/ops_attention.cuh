@@ -334,10 +334,12 @@ struct Attention {
     return p.out + ((size_t)(t.q0 + pos) * p.heads + head * p.group + (row - pos * p.group)) * p.dim;
   }
 
+  // (of a tile that some row sees keys of.  Two tiles: the first may be without, when the causal mask hides every key from it; its
+  // threads wait for nothing and stage their zeros where its queries would be)
   __device__ __forceinline__ static void load_q(const Params &p, const Window &w, const AttnTile &t) {
-    const int tiles = T == 2 && t.npos > p.positions ? 2 : 1;
-    mbar_expect_tx(w.q_bar, (uint32_t)(tiles * w.chunks * p.group * p.positions * 128));
-    for (int x = 0; x < tiles; ++x)
+    const int tiles = T == 2 && t.npos > p.positions ? 2 : 1, first = T == 2 && sub_tile(p, t, 0).keys == 0 ? 1 : 0;
+    mbar_expect_tx(w.q_bar, (uint32_t)((tiles - first) * w.chunks * p.group * p.positions * 128));
+    for (int x = first; x < tiles; ++x)
       for (int ch = 0; ch < w.chunks; ++ch)
         tma_load_3d(w.q + x * w.tile_bytes + ch * kAttnChunkBytes, &p.map_q, w.q_bar, ch * 64, t.head * p.group, t.q0 + x * p.positions);
   }

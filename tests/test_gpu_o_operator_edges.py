@@ -1,0 +1,65 @@
+"""Edges of the language-model operators on the GPU: what a call may ask for that their other tests leave out."""
+import math
+
+import numpy as np
+import pytest
+
+import bfuse_project_b200 as bf
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rt():
+    return bf.Runtime(0)
+
+
+def normal(torch, seed, *shape, mean=0.0, std=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.empty(shape, device="cuda", dtype=torch.bfloat16).normal_(mean, std, generator=g)
+
+
+def offsets(torch, lens):
+    return torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32, device="cuda")
+
+
+def attention(rt, q, k, v, cu_q, cu_kv, out, causal=True):
+    shape = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    d = rt.describe("attention", bf.OP_ATTENTION_BF16, shape, [q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_kv.data_ptr(), out.data_ptr()],
+                    fparam=(q.shape[2] ** -0.5,), flags=bf.flag_share(1) | (bf.FLAG_CAUSAL if causal else 0))
+    return d, rt.register_kernel(d)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_first_tile_of_a_pair_without_keys_is_zero(rt, dim):
+    # two query tiles of 128 positions a CTA.  Where 232, 128 or 200 of a pair's 256 positions come before the first query that
+    # sees a key, its first tile is all behind the mask and its second one is not.  Every launch, every head: exact zeros.
+    import torch
+    kv_lens = [2200, 2100, 2300]
+    q_lens = [kv + n for kv, n in zip(kv_lens, (2 * 256 + 232, 4 * 256 + 128, 6 * 256 + 200))]
+    heads = 24
+    q, k, v = normal(torch, 1, sum(q_lens), heads, dim), normal(torch, 2, sum(kv_lens), heads, dim), normal(torch, 3, sum(kv_lens), heads, dim)
+    cu_q, cu_kv, out = offsets(torch, q_lens), offsets(torch, kv_lens), torch.empty_like(q)
+    d, h = attention(rt, q, k, v, cu_q, cu_kv, out)
+    assert d.shape[9] == 2
+    for _ in range(20):
+        out.fill_(7.0)
+        rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+        assert rt.read_status() == 0
+        q0 = 0
+        for a, b in zip(q_lens, kv_lens):
+            assert (out[q0:q0 + a - b] == 0).all()
+            q0 += a
+    q0 = k0 = 0
+    for a, b in zip(q_lens, kv_lens):       # the first rows with keys, against the definition (tolerance: see the attention tests)
+        n = 200
+        for head in (0, heads - 1):
+            s = q[q0 + a - b:q0 + a - b + n, head].double() @ k[k0:k0 + n, head].double().T * dim ** -0.5
+            p = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf).softmax(-1)
+            vv = v[k0:k0 + n, head].double()
+            want, mag = p @ vv, p @ vv.abs()
+            off = (out[q0 + a - b:q0 + a - b + n, head].double() - want).abs() / (2.0 ** -8 * (mag + want.abs()) + 2.0 ** -14 * mag)
+            assert float(off.max()) <= 1.0, float(off.max())
+        q0, k0 = q0 + a, k0 + b
+    rt.unregister_kernel(h)
