@@ -228,6 +228,9 @@ __global__ void __launch_bounds__(cmax(A::kMaxThreads, B::kMaxThreads), (pair_mi
       } else {
         if (tid < t.n_thr[1]) run_tile<B>(pb, t, 1, vb, tid, 2, smem, 0, queue_tmem_cols > 0, queue_tmem);
       }
+      // what this tile wrote into the window with plain stores (attention stages its rows over the queries) comes before the
+      // next one's TMA loads into the same bytes
+      if constexpr (A::kUsesTmem || B::kUsesTmem) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (t.cta_times && tid == 0) {  // kernel entry, body start (its set-up may overlap the previous kernel), thread 0 done
         t.cta_times[3 * (size_t)ticket] = t_entry;
         t.cta_times[3 * (size_t)ticket + 1] = t_body;

@@ -63,3 +63,33 @@ def test_first_tile_of_a_pair_without_keys_is_zero(rt, dim):
             assert float(off.max()) <= 1.0, float(off.max())
         q0, k0 = q0 + a, k0 + b
     rt.unregister_kernel(h)
+
+
+@pytest.mark.parametrize("dim,lens", [(64, [100] * 90), (128, [300, 40, 0, 700, 1] * 8)])
+def test_work_queue_runs_tile_after_tile_of_attention(rt, dim, lens):
+    # more tiles than resident CTAs: a CTA's next tile loads its queries where the last one's rows were staged
+    import torch
+    stream = torch.cuda.current_stream().cuda_stream
+    cu, heads = offsets(torch, lens), 12
+    sets = []
+    for seed in (1, 5):
+        q, k, v = (normal(torch, seed + i, sum(lens), heads, dim) for i in range(3))
+        sets.append((q, k, v, torch.zeros_like(q)))
+    handles = []
+    for (q, k, v, out), causal in zip(sets, (True, False)):
+        shape = (len(lens), sum(lens), sum(lens), heads, heads, dim)
+        d = rt.describe("attention", bf.OP_ATTENTION_BF16, shape, [t.data_ptr() for t in (q, k, v, cu, cu, out)], fparam=(dim ** -0.5,),
+                        flags=bf.FLAG_CAUSAL if causal else 0)
+        handles.append(rt.register_kernel(d))
+    f = rt.register_fusion(handles[0], handles[1], bf.WORK_QUEUE, 1, 1)
+    rt.launch_sequential(f, stream)
+    assert rt.read_status() == 0
+    want = [s[3].clone() for s in sets]
+    assert all(bool(w.any()) for w in want)
+    for _ in range(10):
+        for s in sets:
+            s[3].fill_(7.0)
+        rt.launch_fused(f, stream)
+        assert rt.read_status() == 0
+        assert all(torch.equal(s[3], w) for s, w in zip(sets, want))
+    rt.unregister_fusion(f)
