@@ -303,14 +303,14 @@ struct ResidualNormBf16 {
     const uint4 *wa4 = p.w_after ? reinterpret_cast<const uint4 *>(p.w_after) + lane : nullptr;
     const uint4 *wb4 = p.w_before ? reinterpret_cast<const uint4 *>(p.w_before) + lane : nullptr;
     const int mine = live ? nv - lane : 0;   // vector i of this thread exists while i * tpr < mine
-    // every load of the row is issued before the first use of any of them (see SoftmaxF32)
+    // every load of the row is issued before the first use of any of them (see SoftmaxF32); r or y may lie over x or b
     uint4 b[kMaxVec], x[kMaxVec];
 #pragma unroll
     for (int i = 0; i < kMaxVec; ++i)
-      if (i * tpr < mine) b[i] = ld_stream_u4(br + i * tpr);
+      if (i * tpr < mine) b[i] = ld_stream_rw_u4(br + i * tpr);
 #pragma unroll
     for (int i = 0; i < kMaxVec; ++i)
-      if (i * tpr < mine) x[i] = ld_stream_u4(xr + i * tpr);
+      if (i * tpr < mine) x[i] = ld_stream_rw_u4(xr + i * tpr);
 #pragma unroll
     for (int i = 0; i < kMaxVec; ++i)
       if (i * tpr < mine) {

@@ -77,6 +77,15 @@ __device__ __forceinline__ uint4 ld_stream_u4(const uint4 *p) {
                : "l"(p));
   return v;
 }
+// As above for memory that this kernel may itself write (an operator that runs in place): .nc is for what nobody writes while it runs.
+__device__ __forceinline__ uint4 ld_stream_rw_u4(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_stream_f4(float4 *p, float4 v) {
   asm volatile("st.global.cs.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");

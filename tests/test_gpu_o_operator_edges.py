@@ -93,3 +93,31 @@ def test_work_queue_runs_tile_after_tile_of_attention(rt, dim, lens):
         assert rt.read_status() == 0
         assert all(torch.equal(s[3], w) for s, w in zip(sets, want))
     rt.unregister_fusion(f)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 8), (300, 264), (700, 1000), (130, 4096), (3, 8192)])
+@pytest.mark.parametrize("norms", [0, 1, 2, 3])
+def test_norms_in_place_give_the_same_bits(rt, rows, cols, norms):
+    # r over x, over the block, y over the other one: rows whose neighbours share their sectors (cols of 8 modulo 16) among them
+    import torch
+    stream = torch.cuda.current_stream().cuda_stream
+    x, b, gate = normal(torch, 1, rows, cols), normal(torch, 2, rows, cols), normal(torch, 3, rows, cols)
+    w = normal(torch, 4, max(1, bin(norms).count("1")), cols, mean=1.0)
+
+    def launched(r, y, px, pb):
+        d = rt.describe("residual_norm", bf.OP_RESIDUAL_NORM_BF16, (rows, cols, norms, 1),
+                        [t.data_ptr() for t in (px, pb, gate)] + [w.data_ptr() if norms else None, r.data_ptr(), y.data_ptr() if y is not None else None],
+                        fparam=(1e-5, 0.5))
+        h = rt.register_kernel(d)
+        rt.launch_kernel(h, stream)
+        assert rt.read_status() == 0
+        rt.unregister_kernel(h)
+        return r, y
+
+    second = norms & bf.NORM_BEFORE
+    r, y = launched(torch.zeros_like(x), torch.zeros_like(x) if second else None, x, b)
+    assert bool(r.any()) and (not second or bool(y.any()))
+    for swap in (False, True):
+        px, pb = x.clone(), b.clone()
+        gr, gy = launched(pb if swap else px, (px if swap else pb) if second else None, px, pb)
+        assert torch.equal(gr, r) and (not second or torch.equal(gy, y))
