@@ -213,9 +213,11 @@ bool is_gemm_umma(int op) { return op == BFUSE_OP_GEMM_TF32 || op == BFUSE_OP_GE
 
 // A GEMM_ACT of few rows runs transposed (GemmUmma::run_few): up to 32 rows by the runtime's choice, or where shape[6] asks for 16
 // or 32 (4 x 4096 x 14336: 22.5 us, 32.0 in tiles of 128 rows; 17 rows 25.9; 33 rows in tiles of 64 30.2, as in tiles of 128).
+// Its ranks share the 128 columns evenly: other numbers of slices that the caller asks for (3 or 5: more do not fit a window)
+// stay with the tiles of 128 rows.
 // The k-slices: while every one finds an SM and keeps eight K blocks -- beside other operators 4 or none.
 bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
-  if (s[6] == 0 ? s[1] > 32 || (s[4] != 0 && s[4] != kUmmaBM) : (s[6] != 16 && s[6] != 32)) return false;
+  if (s[6] == 0 ? s[1] > 32 || (s[4] != 0 && s[4] != kUmmaBM) || (s[5] > 0 && !is_pow2(s[5])) : (s[6] != 16 && s[6] != 32)) return false;
   if (s[6] == 0) *bm = s[1] <= 16 ? 16 : 32;
   if (s[5] > 0) return true;
   const long long tiles = (long long)s[0] * ceil_div(s[1], *bm) * ceil_div(s[2], kUmmaBM) * share;

@@ -121,3 +121,32 @@ def test_norms_in_place_give_the_same_bits(rt, rows, cols, norms):
         px, pb = x.clone(), b.clone()
         gr, gy = launched(pb if swap else px, (px if swap else pb) if second else None, px, pb)
         assert torch.equal(gr, r) and (not second or torch.equal(gy, y))
+
+
+def product(rt, torch, m, n, k, tiling=(0, 0, 0, 0), act=bf.ACT_NONE, other=False, seed=0):
+    a, w, o = normal(torch, seed, m, k), normal(torch, seed + 1, n, k, std=k ** -0.5), normal(torch, seed + 2, m, n) if other else None
+    out = torch.full((m, n), 7.0, device="cuda", dtype=torch.bfloat16)
+    d = rt.describe("gemm_act", bf.OP_GEMM_ACT_BF16, (1, m, n, k) + tuple(tiling), [a.data_ptr(), w.data_ptr(), None, o.data_ptr() if other else None, out.data_ptr()],
+                    flags=bf.flag_share(1) | bf.flag_act(act))
+    h = rt.register_kernel(d)
+    rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+    assert rt.read_status() == 0
+    # the product in fp32 (K 2^-23 of the terms at worst), one rounding
+    z, mag = a.double() @ w.double().T, a.double().abs() @ w.double().abs().T
+    want = z + (o.double() if other else 0)
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + k * 2.0 ** -23 * mag).all()
+    return d, h
+
+
+@pytest.mark.parametrize("split", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("m", [1, 4, 32])
+def test_few_rows_in_any_number_of_k_slices(rt, split, m):
+    import torch
+    if split in (6, 7):      # what so many slices of 128 rows exchange is more than a window, for any number of rows: refused
+        for rows in (m, 33):
+            with pytest.raises(bf.BfuseError, match="shared memory"):
+                product(rt, torch, rows, 264, 4096, (0, split), other=True)
+        return
+    d, h = product(rt, torch, m, 264, 4096, (0, split), other=True)
+    assert d.shape[5] == split and d.shape[6] == (128 if split in (3, 5) else 16 if m <= 16 else 32)
+    rt.unregister_kernel(h)
