@@ -217,7 +217,7 @@ bool is_gemm_umma(int op) { return op == BFUSE_OP_GEMM_TF32 || op == BFUSE_OP_GE
 // stay with the tiles of 128 rows.
 // The k-slices: while every one finds an SM and keeps eight K blocks -- beside other operators 4 or none.
 bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
-  if (s[6] == 0 ? s[1] > 32 || (s[4] != 0 && s[4] != kUmmaBM) || (s[5] > 0 && !is_pow2(s[5])) : (s[6] != 16 && s[6] != 32)) return false;
+  if (s[6] == 0 ? s[1] > 32 || (s[4] != 0 && s[4] != kUmmaBM) || (s[5] > 0 && !is_pow2(s[5])) || s[7] == 2 : (s[6] != 16 && s[6] != 32)) return false;
   if (s[6] == 0) *bm = s[1] <= 16 ? 16 : 32;
   if (s[5] > 0) return true;
   const long long tiles = (long long)s[0] * ceil_div(s[1], *bm) * ceil_div(s[2], kUmmaBM) * share;
@@ -226,6 +226,14 @@ bool gemm_few_rows(const int *s, int share, int sm, int *bm, int *split) {
   for (int c = share == 1 ? 8 : 4; c > 1 && *split == 1; c = share == 1 ? c / 2 : 1)
     if (tiles * c <= sm && num_kb >= 8 * c) *split = c;
   return true;
+}
+
+// What a caller fixes of a GEMM_ACT tiling has to go together: the runtime chooses only what is left 0.
+const char *gemm_form_problem(const int *s) {
+  if (s[7] < 0 || s[7] > 2) return "shape[7] must be 0 (the runtime's choice), 1 (a CTA per tile) or 2 (pairs of CTAs)";
+  if (s[7] == 2 && ((s[4] > 0 && s[4] != 128 && s[4] != 256) || s[5] > 1 || (s[6] > 0 && s[6] != kPairRows))) return "pairs of CTAs take BM = 256, BN = 128 or 256 and one k-slice";
+  if ((s[6] == 16 || s[6] == 32) && s[4] > 0 && s[4] != kUmmaBM) return "BM = 16 or 32 takes BN = 128";
+  return nullptr;
 }
 
 long long gemm_pair_tiles(const int *s, int bn) { return (long long)s[0] * ceil_div(s[1], kPairRows) * ceil_div(s[2], bn); }
@@ -240,7 +248,7 @@ bool gemm_pairs(const int *s, int share, int sm, int *bn) {
   const long long wide = (15 * ((gemm_pair_tiles(s, 256) + slots - 1) / slots)) * kb + 15 * 8;
   const long long narrow = 9 * ((gemm_pair_tiles(s, 128) + slots - 1) / slots) * kb;
   const long long single = 10 * (((long long)s[0] * ceil_div(s[1], kUmmaBM) * ceil_div(s[2], 128) + sm - 1) / sm) * kb;
-  *bn = s[7] == 2 && s[4] != 0 ? s[4] : wide <= narrow ? 256 : 128;
+  *bn = s[7] == 2 && s[4] > 0 ? s[4] : wide <= narrow ? 256 : 128;
   if (s[7] != 0) return s[7] == 2;
   return share == 1 && s[4] == 0 && s[5] == 0 && s[6] == 0 && sm >= 2 && s[3] >= 512 && gemm_pair_tiles(s, *bn) > slots / 2 &&
          std::min(wide, narrow) <= single;
@@ -475,6 +483,9 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0 || s[3] <= 0) { *err = "gemm: batch, M, N, K must be positive"; return BFUSE_ERR_SHAPE; }
       const int eb = d->op == BFUSE_OP_GEMM_TF32 ? 4 : 2;
       int bn = s[4], split = s[5], bm = s[6], q;
+      if (d->op == BFUSE_OP_GEMM_ACT_BF16) {
+        if (const char *m = gemm_form_problem(s)) { *err = std::string("gemm: ") + m; return BFUSE_ERR_SHAPE; }
+      }
       if (d->op == BFUSE_OP_GEMM_ACT_BF16 && gemm_few_rows(s, share, sm, &bm, &split)) {
         const int num_kb = ceil_div(s[3] * eb, kUmmaRowBytes);
         if (split > num_kb || (split & (split - 1)) || split > 8) { *err = "gemm: a tile of few rows takes 1, 2, 4 or 8 k-slices, at most the number of K blocks"; return BFUSE_ERR_SHAPE; }
@@ -490,7 +501,6 @@ int default_launch(const bfuse_context *ctx, bfuse_kernel_desc *d, std::string *
       }
       if (d->op == BFUSE_OP_GEMM_ACT_BF16) {
         if (int wide; gemm_pairs(s, share, sm, &wide)) {
-          if (wide != 128 && wide != 256) { *err = "gemm: pairs of CTAs take BN = 128 or 256"; return BFUSE_ERR_SHAPE; }
           const long long tiles = gemm_pair_tiles(s, wide);
           d->shape[4] = wide, d->shape[5] = 1, d->shape[6] = kPairRows, d->shape[7] = 2;
           set(2 * (int)std::min<long long>(tiles, sm / 2), 1, 1, kUmmaThreads, 1, pair_smem_bytes(wide), 5);

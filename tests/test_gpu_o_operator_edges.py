@@ -150,3 +150,11 @@ def test_few_rows_in_any_number_of_k_slices(rt, split, m):
     d, h = product(rt, torch, m, 264, 4096, (0, split), other=True)
     assert d.shape[5] == split and d.shape[6] == (128 if split in (3, 5) else 16 if m <= 16 else 32)
     rt.unregister_kernel(h)
+
+
+def test_pairs_of_ctas_asked_for_with_few_rows(rt):
+    import torch
+    for m in (1, 32):
+        d, h = product(rt, torch, m, 264, 1096, (0, 0, 0, 2), other=True)
+        assert d.shape[6] == 256 and d.shape[7] == 2
+        rt.unregister_kernel(h)

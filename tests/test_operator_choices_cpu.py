@@ -28,3 +28,19 @@ def test_k_slices_that_no_tile_takes():
     assert gemm(1, 4, 4096, 4096, 0, 9)[0] == SHAPE_ERR
     assert gemm(1, 4, 4096, 256, 0, 8)[0] == SHAPE_ERR     # four K blocks
     assert gemm(1, 4, 4096, 4096, 0, 3, 16)[0] == SHAPE_ERR
+
+
+def test_a_tiling_that_is_asked_for_is_used():
+    assert gemm(1, 16, 4096, 4096, 0, 0, 0, 2)[1] == (128, 1, 256, 2)         # pairs of CTAs for few rows, too (32 narrow tiles for 74 pairs)
+    assert gemm(1, 16, 4096, 4096, 256, 0, 0, 2)[1] == (256, 1, 256, 2)
+    assert gemm(1, 16, 4096, 4096, -1, 0, 0, 2)[1][0] in (128, 256)
+    assert gemm(1, 16, 4096, 4096, 0, 0, 0, 1)[1][2:] == (16, 1)
+    for tiling in ((256, 1, 256, 2), (128, 1, 256, 2), (128, 4, 16, 1), (128, 1, 32, 1), (64, 2, 128, 1)):   # written back: the same again
+        assert gemm(1, 30, 4096, 4096, *tiling) == (0, tiling)
+
+
+@pytest.mark.parametrize("tiling", [(64, 1, 16), (256, 2, 32), (0, 0, 16, 2), (0, 0, 32, 2), (256, 4, 0, 2), (256, 1, 128, 2), (0, 2, 256, 2), (0, 0, 0, 3),
+                                    (0, 0, 0, -1)])
+def test_a_tiling_that_no_kernel_runs_is_refused(tiling):
+    for m in (4, 32, 300):
+        assert gemm(1, m, 4096, 4096, *tiling)[0] == SHAPE_ERR
