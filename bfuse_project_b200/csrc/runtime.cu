@@ -2016,6 +2016,8 @@ int bfuse_debug_gemm_timeline(bfuse_context *ctx, int kernel, long long *marks, 
   const bool is_conv = k->desc.op == BFUSE_OP_CONV2D_TF32;
   if (!is_gemm_umma(k->desc.op) && !is_conv)
     return fail(ctx, BFUSE_ERR_UNSUPPORTED, "only the tcgen05 GEMM / conv bodies record a timeline");
+  if (k->desc.op == BFUSE_OP_GEMM_ACT_BF16 && (k->desc.shape[7] == 2 || (k->desc.shape[6] > 0 && umma_few_rows(k->desc.shape[6]))))
+    return fail(ctx, BFUSE_ERR_UNSUPPORTED, "GEMM_ACT in pairs of CTAs or in tiles of 16 or 32 rows records no timeline");
   cudaSetDevice(ctx->device);
   long long *d = nullptr;
   const int held = std::max(n, (int)MARK_COUNT);

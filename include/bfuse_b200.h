@@ -249,7 +249,8 @@ int bfuse_trace_fused(bfuse_context *ctx, int fusion, int *kernel_of, int *vbloc
 /* Diagnostic, no reference counterpart: run a registered tcgen05 GEMM kernel once (unfused) with its
  * first CTA recording global-timer marks in nanoseconds: start, set-up done, first / last TMA load
  * issued, first stage full, last MMA issued, accumulator ready, partial tile written, cluster
- * barrier 1, reduction done, cluster barrier 2, end (12 values; unused marks stay 0). Synchronises. */
+ * barrier 1, reduction done, cluster barrier 2, end (12 values; unused marks stay 0). Synchronises.  GEMM_ACT kernels of
+ * pairs of CTAs or of tiles of 16 or 32 rows have no marks: BFUSE_ERR_UNSUPPORTED. */
 int bfuse_debug_gemm_timeline(bfuse_context *ctx, int kernel, long long *marks, int n);
 /* Diagnostic, no reference counterpart: launch the n block-level fusions back to back on the
  * context's stream (fused mode), every dispatch slot (as in bfuse_fusion_map_block; the blocks of a run share their

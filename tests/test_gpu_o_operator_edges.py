@@ -158,3 +158,16 @@ def test_pairs_of_ctas_asked_for_with_few_rows(rt):
         d, h = product(rt, torch, m, 264, 1096, (0, 0, 0, 2), other=True)
         assert d.shape[6] == 256 and d.shape[7] == 2
         rt.unregister_kernel(h)
+
+
+def test_timeline_of_a_form_that_records_none_is_refused(rt):
+    import torch
+    for tiling in ((0, 0, 16), (0, 0, 0, 2)):
+        d, h = product(rt, torch, 16, 264, 1096, tiling)
+        with pytest.raises(bf.BfuseError, match="timeline"):
+            rt.gemm_timeline(h)
+        rt.unregister_kernel(h)
+    d, h = product(rt, torch, 16, 264, 1096, (128, 1, 128))
+    marks = rt.gemm_timeline(h)
+    assert marks["end"] >= marks["acc_ready"] >= marks["setup_done"] >= 0 and marks["end"] > 0
+    rt.unregister_kernel(h)
