@@ -171,3 +171,50 @@ def test_timeline_of_a_form_that_records_none_is_refused(rt):
     marks = rt.gemm_timeline(h)
     assert marks["end"] >= marks["acc_ready"] >= marks["setup_done"] >= 0 and marks["end"] > 0
     rt.unregister_kernel(h)
+
+
+def activation(torch, act, z):
+    if act == bf.ACT_GELU:
+        return z * torch.special.log_ndtr(z).exp()
+    if act == bf.ACT_GELU_TANH:
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z * torch.sigmoid(z)
+
+
+@pytest.mark.parametrize("form", [(128, 1, 128, 1), (128, 1, 16, 1), (256, 1, 256, 2)])
+@pytest.mark.parametrize("act,lowest", [(bf.ACT_GELU, -14.0)])
+def test_tails_of_the_activations(rt, act, lowest, form):
+    # The product is 0, so the bias alone is activated: as it is, in fp32.  Against 64 bits, relative to the value: the activation
+    # within 2^-16 (a few 2^-24 of the exponent, which is 126 / log2(e) at most: 2^-17; the rest 2^-20), half a step of bf16 (2^-8), and
+    # nothing finer than the smallest normal value (2^-126).
+    import torch
+    n, k = 8192, 64
+    z = torch.cat([torch.linspace(lowest, 0, n // 2, device="cuda"), torch.linspace(0, -lowest, n // 2, device="cuda")]).contiguous()
+    for m in (1, 16):
+        a, w = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16), normal(torch, 1, n, k)
+        out = torch.full((m, n), 7.0, device="cuda", dtype=torch.bfloat16)
+        d = rt.describe("gemm_act", bf.OP_GEMM_ACT_BF16, (1, m, n, k) + form, [a.data_ptr(), w.data_ptr(), z.data_ptr(), None, out.data_ptr()],
+                        flags=bf.flag_share(1) | bf.flag_act(act))
+        h = rt.register_kernel(d)
+        rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+        assert rt.read_status() == 0
+        want = activation(torch, act, z.double())
+        off = (out.double() - want).abs() / ((2.0 ** -8 + 2.0 ** -16) * want.abs() + 2.0 ** -126)
+        assert float(off.max()) <= 1.0, (float(off.max()), float(z[off.max(0).values.argmax()]))
+        rt.unregister_kernel(h)
+
+
+@pytest.mark.parametrize("act", [bf.ACT_RELU, bf.ACT_GELU, bf.ACT_GELU_TANH, bf.ACT_SILU])
+def test_activations_of_huge_values_and_nan(rt, act):
+    import torch
+    z = torch.tensor([math.inf, 3e38, 1e30, 100.0, -100.0, -1e30, -3e38, math.nan], device="cuda")
+    for form in ((128, 1, 128, 1), (128, 1, 16, 1)):
+        a, w = torch.zeros(2, 64, device="cuda", dtype=torch.bfloat16), normal(torch, 1, 8, 64)
+        out = torch.full((2, 8), 7.0, device="cuda", dtype=torch.bfloat16)
+        h = rt.register_kernel(rt.describe("gemm_act", bf.OP_GEMM_ACT_BF16, (1, 2, 8, 64) + form, [a.data_ptr(), w.data_ptr(), z.data_ptr(), None, out.data_ptr()],
+                                           flags=bf.flag_share(1) | bf.flag_act(act)))
+        rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+        assert rt.read_status() == 0
+        for row in out.float():
+            assert torch.equal(row[:4], z[:4].to(torch.bfloat16).float()) and (row[4:7] == 0).all() and bool(row[7].isnan())
+        rt.unregister_kernel(h)
