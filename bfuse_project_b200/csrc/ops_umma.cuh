@@ -261,17 +261,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// x / (1 + 2^-z)
-__device__ __forceinline__ float2 over_one_plus_exp2(float2 x, float2 z) {
-  return mul2(x, make_float2(rcp_approx(1.f + exp2_approx(-z.x)), rcp_approx(1.f + exp2_approx(-z.y))));
+// x / (1 + 2^-z), of y = -8 - z: the sum is taken 2^-8 smaller, so that its reciprocal leaves the normal range only where the
+// result does (SiLU: below -92; with the sum as it is at -87, which lost values of up to 5e-37)
+__device__ __forceinline__ float2 over_one_plus_exp2(float2 x, float2 y) {
+  constexpr float k = 1.f / 256.f;
+  return mul2(mul2(x, make_float2(k, k)), make_float2(rcp_approx(k + exp2_approx(y.x)), rcp_approx(k + exp2_approx(y.y))));
 }
 template <int ACT>
 __device__ __forceinline__ float2 activate(float2 x) {
+  const float2 m8 = make_float2(-8.f, -8.f);
   if (ACT == ACT_RELU) return make_float2(x.x > 0.f ? x.x : (x.x != x.x ? x.x : 0.f), x.y > 0.f ? x.y : (x.y != x.y ? x.y : 0.f));
-  if (ACT == ACT_SILU) return over_one_plus_exp2(x, mul2(x, make_float2(1.4426950408889634f, 1.4426950408889634f)));
+  if (ACT == ACT_SILU) return over_one_plus_exp2(x, fma2(x, make_float2(-1.4426950408889634f, -1.4426950408889634f), m8));
   if (ACT == ACT_GELU_TANH) {   // 1/2 (1 + tanh u) = 1 / (1 + e^-2u), u = sqrt(2 / pi) (x + 0.044715 x^3)
-    constexpr float a = 2.302208198f, b = 0.10294324f;   // 2 sqrt(2 / pi) log2(e), and 0.044715 times that
-    return over_one_plus_exp2(x, mul2(x, fma2(mul2(x, x), make_float2(b, b), make_float2(a, a))));
+    constexpr float a = -2.302208198f, b = -0.10294324f;   // -2 sqrt(2 / pi) log2(e), and 0.044715 times that
+    return over_one_plus_exp2(x, fma2(x, fma2(mul2(x, x), make_float2(b, b), make_float2(a, a)), m8));
   }
   if (ACT == ACT_GELU) {
     // x Phi(x) = max(x, 0) - a Phi(-a), a = |x|.  Phi(-a) = e^(-a^2 / 2) R(a) with R(a) = erfcx(a / sqrt(2)) / 2 = t (c1 + ... + c8 t^7),

@@ -135,7 +135,7 @@ def product(rt, torch, m, n, k, tiling=(0, 0, 0, 0), act=bf.ACT_NONE, other=Fals
     z, mag = a.double() @ w.double().T, a.double().abs() @ w.double().abs().T
     want = z + (o.double() if other else 0)
     assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + k * 2.0 ** -23 * mag).all()
-    return d, h
+    return d, h, (a, w, o, out)
 
 
 @pytest.mark.parametrize("split", [1, 2, 3, 4, 5, 6, 7, 8])
@@ -147,7 +147,7 @@ def test_few_rows_in_any_number_of_k_slices(rt, split, m):
             with pytest.raises(bf.BfuseError, match="shared memory"):
                 product(rt, torch, rows, 264, 4096, (0, split), other=True)
         return
-    d, h = product(rt, torch, m, 264, 4096, (0, split), other=True)
+    d, h, _ = product(rt, torch, m, 264, 4096, (0, split), other=True)
     assert d.shape[5] == split and d.shape[6] == (128 if split in (3, 5) else 16 if m <= 16 else 32)
     rt.unregister_kernel(h)
 
@@ -155,7 +155,7 @@ def test_few_rows_in_any_number_of_k_slices(rt, split, m):
 def test_pairs_of_ctas_asked_for_with_few_rows(rt):
     import torch
     for m in (1, 32):
-        d, h = product(rt, torch, m, 264, 1096, (0, 0, 0, 2), other=True)
+        d, h, _ = product(rt, torch, m, 264, 1096, (0, 0, 0, 2), other=True)
         assert d.shape[6] == 256 and d.shape[7] == 2
         rt.unregister_kernel(h)
 
@@ -163,11 +163,11 @@ def test_pairs_of_ctas_asked_for_with_few_rows(rt):
 def test_timeline_of_a_form_that_records_none_is_refused(rt):
     import torch
     for tiling in ((0, 0, 16), (0, 0, 0, 2)):
-        d, h = product(rt, torch, 16, 264, 1096, tiling)
+        _, h, buffers = product(rt, torch, 16, 264, 1096, tiling)
         with pytest.raises(bf.BfuseError, match="timeline"):
             rt.gemm_timeline(h)
         rt.unregister_kernel(h)
-    d, h = product(rt, torch, 16, 264, 1096, (128, 1, 128))
+    _, h, buffers = product(rt, torch, 16, 264, 1096, (128, 1, 128))
     marks = rt.gemm_timeline(h)
     assert marks["end"] >= marks["acc_ready"] >= marks["setup_done"] >= 0 and marks["end"] > 0
     rt.unregister_kernel(h)
@@ -182,7 +182,7 @@ def activation(torch, act, z):
 
 
 @pytest.mark.parametrize("form", [(128, 1, 128, 1), (128, 1, 16, 1), (256, 1, 256, 2)])
-@pytest.mark.parametrize("act,lowest", [(bf.ACT_GELU, -14.0)])
+@pytest.mark.parametrize("act,lowest", [(bf.ACT_GELU, -14.0), (bf.ACT_GELU_TANH, -10.5), (bf.ACT_SILU, -95.0)])
 def test_tails_of_the_activations(rt, act, lowest, form):
     # The product is 0, so the bias alone is activated: as it is, in fp32.  Against 64 bits, relative to the value: the activation
     # within 2^-16 (a few 2^-24 of the exponent, which is 126 / log2(e) at most: 2^-17; the rest 2^-20), half a step of bf16 (2^-8), and
