@@ -218,3 +218,120 @@ def test_activations_of_huge_values_and_nan(rt, act):
         for row in out.float():
             assert torch.equal(row[:4], z[:4].to(torch.bfloat16).float()) and (row[4:7] == 0).all() and bool(row[7].isnan())
         rt.unregister_kernel(h)
+
+
+@pytest.mark.parametrize("form", [(64, 1, 128, 1), (128, 4, 128, 1), (256, 1, 256, 1), (128, 1, 16, 1), (128, 8, 32, 1), (256, 1, 256, 2), (128, 1, 256, 2)])
+@pytest.mark.parametrize("mul", [False, True])
+def test_products_in_place_give_the_same_bits(rt, form, mul):
+    # the residual (or the factor) is the output, in every form of the product
+    import torch
+    m, n, k = 300, 520, 1096
+    a, w, other = normal(torch, 1, 2, m, k), normal(torch, 2, 2, n, k, std=k ** -0.5), normal(torch, 3, 2, m, n)
+    outs = []
+    for src, dst in ((other, torch.zeros_like(other)), (other.clone(), None)):
+        dst = src if dst is None else dst
+        h = rt.register_kernel(rt.describe("gemm_act", bf.OP_GEMM_ACT_BF16, (2, m, n, k) + form, [a.data_ptr(), w.data_ptr(), None, src.data_ptr(), dst.data_ptr()],
+                                           flags=bf.flag_share(1) | bf.flag_act(bf.ACT_SILU) | (bf.FLAG_MUL if mul else 0)))
+        rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+        assert rt.read_status() == 0
+        rt.unregister_kernel(h)
+        outs.append(dst)
+    assert bool(outs[0].any()) and torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("seqs", [3, 12, 40])
+def test_caches_with_room_to_grow(rt, seqs):
+    # a sequence without queries owns the room behind each cache; what lies there does not matter, and the offsets move as caches grow
+    import torch
+    heads, kvh, dim, room = 8, 2, 64, 400
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(1, room, seqs)]
+    q, k, v = normal(torch, 1, seqs, heads, dim), normal(torch, 2, seqs * room, kvh, dim), normal(torch, 3, seqs * room, kvh, dim)
+    cu_q = torch.tensor([0] + [i // 2 + 1 for i in range(2 * seqs)], dtype=torch.int32, device="cuda")
+    cu_kv, out = torch.zeros(2 * seqs + 1, dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    _, h = attention(rt, q, k, v, cu_q, cu_kv, out)
+    keep_k, keep_v = k.clone(), v.clone()
+    for step in range(3):
+        ends = [x for i, n in enumerate(lens) for x in (i * room + n, (i + 1) * room)]
+        cu_kv.copy_(torch.tensor([0] + ends, dtype=torch.int32))
+        for i, n in enumerate(lens):
+            k[i * room:(i + 1) * room], v[i * room:(i + 1) * room] = keep_k[i * room:(i + 1) * room], keep_v[i * room:(i + 1) * room]
+            k[i * room + n:(i + 1) * room], v[i * room + n:(i + 1) * room] = math.nan, math.inf
+        out.fill_(7.0)
+        rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+        assert rt.read_status() == 0
+        for i, n in enumerate(lens):
+            kk, vv = (t[i * room:i * room + n].double().repeat_interleave(heads // kvh, 1) for t in (keep_k, keep_v))
+            p = (torch.einsum("hd,khd->hk", q[i].double(), kk) * dim ** -0.5).softmax(-1)
+            want, mag = torch.einsum("hk,khd->hd", p, vv), torch.einsum("hk,khd->hd", p, vv.abs())
+            off = (out[i].double() - want).abs() / (2.0 ** -8 * (mag + want.abs()) + 2.0 ** -14 * mag)
+            assert float(off.max()) <= 1.0, float(off.max())
+        lens = [min(room, n + 1) for n in lens]
+    rt.unregister_kernel(h)
+
+
+def test_offsets_that_pass_32_bits(rt):
+    # 2.3e9 elements of keys, of values, of queries and of the output: bytes and elements past 32 and 31 bits
+    import torch
+    kvh, dim, tokens = 8, 128, 2_250_000
+    k, v = (torch.empty(tokens, kvh, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    k[-700:], v[-700:] = normal(torch, 1, 700, kvh, dim), normal(torch, 2, 700, kvh, dim)
+    q = normal(torch, 3, 2, 4 * kvh, dim)
+    cu_q, cu_kv = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), torch.tensor([tokens - 700, tokens - 300, tokens], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+
+    def check(got, qq, kk, vv):
+        kk, vv = (t.double().repeat_interleave(qq.shape[0] // t.shape[1], 1) for t in (kk, vv))
+        p = (torch.einsum("hd,khd->hk", qq.double(), kk) * dim ** -0.5).softmax(-1)
+        want, mag = torch.einsum("hk,khd->hd", p, vv), torch.einsum("hk,khd->hd", p, vv.abs())
+        assert ((got.double() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) + 2.0 ** -14 * mag).all()
+
+    _, h = attention(rt, q, k, v, cu_q, cu_kv, out)
+    rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+    assert rt.read_status() == 0
+    check(out[0], q[0], k[-700:-300], v[-700:-300])
+    check(out[1], q[1], k[-300:], v[-300:])
+    rt.unregister_kernel(h)
+    # the same buffers as queries and output: one key for all but the last three positions
+    q, out, keys, values = k, v, normal(torch, 4, 4, kvh, dim), normal(torch, 5, 4, kvh, dim)
+    q[-3:] = normal(torch, 6, 3, kvh, dim)
+    q[:-3].zero_()
+    cu_q, cu_kv = torch.tensor([0, tokens - 3, tokens], dtype=torch.int32, device="cuda"), torch.tensor([0, 1, 4], dtype=torch.int32, device="cuda")
+    out.fill_(7.0)
+    _, h = attention(rt, q, keys, values, cu_q, cu_kv, out, causal=False)
+    rt.launch_kernel(h, torch.cuda.current_stream().cuda_stream)
+    assert rt.read_status() == 0
+    for i in (-3, -2, -1):
+        check(out[i], q[i], keys[1:], values[1:])
+    assert torch.equal(out[:-3:100_000], values[:1].expand_as(out[:-3:100_000])) and torch.equal(out[-5], values[0])
+    rt.unregister_kernel(h)
+
+
+@pytest.mark.parametrize("pattern", [bf.ZIGZAG, bf.PROPORTIONAL, bf.SM_STRIPED, bf.THREAD_SPLIT, bf.RANGE_SPLIT, bf.WORK_QUEUE])
+def test_fused_norms_against_the_definition(rt, pattern):
+    # (two roundings of 2^-8 at most: r's, and y's; fp32 adds less than 2^-16 of the terms)
+    import torch
+    stream, eps, scale = torch.cuda.current_stream().cuda_stream, 1e-5, 0.5
+    sets, handles = [], []
+    for seed, (rows, cols) in enumerate(((700, 4096), (333, 768))):
+        x, b, w = normal(torch, 10 * seed, rows, cols), normal(torch, 10 * seed + 1, rows, cols), normal(torch, 10 * seed + 2, 2, cols, mean=1.0)
+        r, y = torch.zeros_like(x), torch.zeros_like(x)
+        d = rt.describe("residual_norm", bf.OP_RESIDUAL_NORM_BF16, (rows, cols, bf.NORM_AFTER | bf.NORM_BEFORE, 0),
+                        [x.data_ptr(), b.data_ptr(), None, w.data_ptr(), r.data_ptr(), y.data_ptr()], fparam=(eps, scale))
+        handles.append(rt.register_kernel(d))
+        sets.append((x, b, w, r, y))
+    f = rt.register_fusion(handles[0], handles[1], pattern, 1, 1)
+    for launch in (rt.launch_sequential, rt.launch_fused):
+        for *_, r, y in sets:
+            r.zero_(), y.zero_()
+        launch(f, stream)
+        assert rt.read_status() == 0
+        for x, b, w, r, y in sets:
+            x, b, w = x.double(), b.double(), w.double()
+            n = scale * b / (b.pow(2).mean(1, keepdim=True) + eps).sqrt() * w[0]
+            want, mag = x + n, x.abs() + n.abs()
+            inv = 1 / (want.pow(2).mean(1, keepdim=True) + eps).sqrt()
+            assert ((r.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * mag).all()
+            y_want = want * inv * w[1]
+            assert ((y.double() - y_want).abs() <= 2.0 ** -8 * y_want.abs() + 2.0 ** -16 * (mag * inv * w[1].abs() + y_want.abs())).all()
+    rt.unregister_fusion(f)
