@@ -335,3 +335,36 @@ def test_fused_norms_against_the_definition(rt, pattern):
             y_want = want * inv * w[1]
             assert ((y.double() - y_want).abs() <= 2.0 ** -8 * y_want.abs() + 2.0 ** -16 * (mag * inv * w[1].abs() + y_want.abs())).all()
     rt.unregister_fusion(f)
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 264), (700, 1000), (40, 8)])
+def test_in_place_stream_of_layers(rt, rows, cols):
+    # a residual stream updated in place and read by the next launch, which starts under this one's tail: rows that share a sector
+    import torch
+    stream, layers = torch.cuda.current_stream().cuda_stream, 24
+    x, b, w = normal(torch, 1, rows, cols), normal(torch, 2, layers, rows, cols), normal(torch, 3, 2, cols, mean=1.0)
+    ys = torch.zeros(layers, rows, cols, device="cuda", dtype=torch.bfloat16)
+
+    def layer(i, r):
+        return rt.register_kernel(rt.describe("residual_norm", bf.OP_RESIDUAL_NORM_BF16, (rows, cols, bf.NORM_AFTER | bf.NORM_BEFORE, 0),
+                                              [x.data_ptr(), b[i].data_ptr(), None, w.data_ptr(), r.data_ptr(), ys[i].data_ptr()], fparam=(1e-5, 0.5)))
+
+    start, other = x.clone(), torch.zeros_like(x)
+    for i in range(layers):      # out of place, one launch at a time
+        h = layer(i, other)
+        rt.launch_kernel(h, stream)
+        torch.cuda.synchronize()
+        x.copy_(other)
+        torch.cuda.synchronize()
+        rt.unregister_kernel(h)
+    want = x.clone(), ys.clone()
+    handles = [layer(i, x) for i in range(layers)]
+    for _ in range(10):
+        x.copy_(start)
+        ys.zero_()
+        for h in handles:
+            rt.launch_kernel(h, stream)
+        assert rt.read_status() == 0
+        assert torch.equal(x, want[0]) and torch.equal(ys, want[1])
+    for h in handles:
+        rt.unregister_kernel(h)
